@@ -6,6 +6,7 @@ Importing fails if libclq.so has not been built: there is no CPU path.
 """
 from . import _lib
 from ._lib import ClqError
+from .int8 import Int8Rows, linear_int8, norm_quantize, quantize_rows, swiglu_quantize
 from .quant import (DTYPES, PackedDtype, PackedError, PackedStorage, PackedTensor,
                     UnsupportedOperation, astype, copy_tensor, dequantize, find_dtype, linear,
                     make_packed_storage, make_q4_0_storage, make_q4_k_storage, make_q6_k_storage,
@@ -14,9 +15,10 @@ from .quant import (DTYPES, PackedDtype, PackedError, PackedStorage, PackedTenso
 from .store import Store, linear_fused, linear_group, linear_group_fused
 
 __all__ = [
-    "ClqError", "DTYPES", "PackedDtype", "PackedError", "PackedStorage", "PackedTensor", "Store",
+    "ClqError", "DTYPES", "Int8Rows", "PackedDtype", "PackedError", "PackedStorage", "PackedTensor", "Store",
     "UnsupportedOperation", "astype", "copy_tensor", "dequantize", "find_dtype", "linear",
-    "make_packed_storage", "make_q4_0_storage", "make_q4_k_storage", "make_q6_k_storage",
-    "make_q8_0_storage", "make_tensor_view", "matmul", "slice_rows", "take", "take_dequantized",
+    "linear_int8", "make_packed_storage", "make_q4_0_storage", "make_q4_k_storage", "make_q6_k_storage",
+    "make_q8_0_storage", "make_tensor_view", "matmul", "norm_quantize", "quantize_rows",
+    "slice_rows", "swiglu_quantize", "take", "take_dequantized",
     "transpose", "linear_group",
 ]

@@ -87,6 +87,13 @@ SIGNATURES = {
     "clq_kv_cache_status": (_int, [_ptr, ctypes.POINTER(_int)]),
     "clq_kv_cache_read": (_int, [_ptr, _int, _i64, _ptr, _ptr, _ptr]),
     "clq_rope_device": (_int, [_ptr, _i64, _int, _int, _i64, _i64, _int, _i64, ctypes.c_double, _ptr, _int, _ptr]),
+    "clq_quantize_rows_device": (_int, [_ptr, _int, _i64, _i64, _i64, _ptr, _i64, _ptr, _ptr]),
+    "clq_norm_quantize_device": (_int, [_ptr, _int, _i64, _i64, _i64, _ptr, ctypes.c_float, _ptr, _int, _i64, _ptr, _i64,
+                                        _ptr, _i64, _ptr, _ptr]),
+    "clq_swiglu_quantize_device": (_int, [_ptr, _i64, _ptr, _i64, _int, _i64, _i64, _ptr, _i64, _ptr, _ptr]),
+    "clq_dequantize_rows_device": (_int, [_ptr, _i64, _ptr, _i64, _i64, _ptr, _int, _i64, _ptr]),
+    "clq_linear_int8_device": (_int, [_ptr, _i64, _ptr, _i64, _ptr, _i64, _ptr, _i64, _i64, _ptr, _i64, _ptr, _int, _i64,
+                                      _ptr]),
     "clq_attend_device": (_int, [_ptr, _i64, _int, _i64, _ptr, _int, _i64, _i64, _ptr, _i64, _ptr]),
 }
 

@@ -331,6 +331,8 @@ int cached_store(int dtype, int64_t n, int64_t k, const uint8_t* bytes, int devi
 
 }  // namespace
 
+int clq::sm100_device(int* dev) { return current_device(dev); }
+
 int clq::set_error(int code, const char* fmt, ...) {
     char buf[512];
     va_list ap;

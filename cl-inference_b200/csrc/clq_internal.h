@@ -23,6 +23,9 @@ bool geometry(int dtype, int* elems, int* block_bytes);
 
 // Records the formatted message as this thread's clq_last_error and returns CODE.
 int set_error(int code, const char* fmt, ...);
+// The current device, which must be an sm_100 part (checked once per device);
+// a CLQ_ERR_* code otherwise.
+int sm100_device(int* dev);
 // Makes the current device's stream-ordered pool keep released memory (once per device).
 cudaError_t keep_pool_memory();
 
@@ -164,5 +167,48 @@ bool uses_gemm_tc(const WeightView& w, int xtype, int64_t m, unsigned flags);
 // The generic (any alignment, any M) kernel, also used as a fallback by launch_linear.
 cudaError_t launch_linear_generic(const WeightView& w, int64_t rows, const void* x, int xtype,
                                   int64_t m, float* out, int64_t ldo, cudaStream_t stream);
+
+// ---- 8-bit rows (int8_rows.cu, int8_linear.cu, int8_gemm.cu) ----------------
+// M rows of K elements of XTYPE to codes and one scale a row: v = x, silu(gate) *
+// x with a gate, (x + res) * norm_w with a residual / norm weight (null: absent).
+// Strides in elements; res and res_out have RTYPE (XTYPE or f32).
+struct QuantRows {
+    const void* x;
+    int xtype;
+    int64_t m, k, ldx;
+    const void* gate;
+    int64_t ldg;
+    const float* norm_w;
+    float eps;
+    const void* res;
+    int rtype;
+    int64_t ldr;
+    void* res_out;
+    int64_t ldro;
+    int8_t* codes;
+    int64_t ldc;
+    float* scales;
+};
+cudaError_t launch_quantize_rows(const QuantRows& q, cudaStream_t stream);
+cudaError_t launch_dequantize_rows(const int8_t* codes, int64_t ldc, const float* scales, int64_t m, int64_t k, void* out,
+                                   int otype, int64_t ldo, cudaStream_t stream);
+// out [m, n] of OTYPE = x [m, k] w [n, k]^T with a scale for each row of both,
+// plus an optional f32 residual (which OUT may be).
+struct Int8Product {
+    const int8_t* x;
+    int64_t ldx;
+    const float* xs;
+    int64_t m;
+    const int8_t* w;
+    int64_t ldw;
+    const float* ws;
+    int64_t n, k;
+    const float* res;
+    int64_t ldr;
+    void* out;
+    int otype;
+    int64_t ldo;
+};
+cudaError_t launch_linear_int8(const Int8Product& p, cudaStream_t stream);
 
 }  // namespace clq

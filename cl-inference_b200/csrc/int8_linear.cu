@@ -1,0 +1,211 @@
+// int8_linear.cu -- the product of 8-bit rows (int8_rows.cu):
+//   out[t, j] = round(float(sum_c x[t, c] * w[j, c]) * (w scale j) * (x scale t) + residual[t, j])
+// with the sum in 32-bit integers, so it is exact and the same however it is
+// split.  This file holds the C entry points of the 8-bit operators, the
+// choice of a kernel, and the kernel for operands that no wide load can read.
+#include <cstdint>
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include "../../include/clq.h"
+#include "clq_internal.h"
+
+namespace clq {
+namespace {
+
+__device__ __forceinline__ void store_out(void* out, int otype, int64_t i, float v) {
+    if (otype == CLQ_X_F32) static_cast<float*>(out)[i] = v;
+    else if (otype == CLQ_X_BF16) static_cast<__nv_bfloat16*>(out)[i] = __float2bfloat16_rn(v);
+    else static_cast<__half*>(out)[i] = __float2half_rn(v);
+}
+
+// A CTA forms 64 x 64 outputs, 4 x 4 a thread, from 32-byte columns of both
+// operands staged in shared memory a byte at a time (any base and stride),
+// four products to an instruction.
+constexpr int kGT = 64, kGK = 32;
+__global__ void __launch_bounds__(256) linear_int8_generic_kernel(const Int8Product P) {
+    __shared__ int xs[kGK / 4][kGT + 1], ws[kGK / 4][kGT + 1];
+    const int64_t t0 = (int64_t)blockIdx.y * kGT, n0 = (int64_t)blockIdx.x * kGT;
+    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+    int acc[4][4] = {};
+    for (int64_t k0 = 0; k0 < P.k; k0 += kGK) {
+        for (int e = threadIdx.x; e < kGT * kGK / 4; e += 256) {
+            const int r = e / (kGK / 4), c = e % (kGK / 4);
+            uint32_t a = 0, b = 0;
+            for (int i = 0; i < 4; i++) {
+                const int64_t kk = k0 + 4 * c + i;
+                if (kk < P.k && t0 + r < P.m) a |= (uint32_t)(uint8_t)P.x[(t0 + r) * P.ldx + kk] << (8 * i);
+                if (kk < P.k && n0 + r < P.n) b |= (uint32_t)(uint8_t)P.w[(n0 + r) * P.ldw + kk] << (8 * i);
+            }
+            xs[c][r] = (int)a;
+            ws[c][r] = (int)b;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int c = 0; c < kGK / 4; c++)
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+#pragma unroll
+                for (int j = 0; j < 4; j++) acc[i][j] = __dp4a(xs[c][ty + 16 * i], ws[c][tx + 16 * j], acc[i][j]);
+        __syncthreads();
+    }
+    for (int i = 0; i < 4; i++)
+        for (int j = 0; j < 4; j++) {
+            const int64_t t = t0 + ty + 16 * i, n = n0 + tx + 16 * j;
+            if (t >= P.m || n >= P.n) continue;
+            float v = __fmul_rn(__fmul_rn((float)acc[i][j], P.ws[n]), P.xs[t]);
+            if (P.res) v = __fadd_rn(v, P.res[t * P.ldr + n]);
+            store_out(P.out, P.otype, t * P.ldo + n, v);
+        }
+}
+
+cudaError_t launch_linear_int8_generic(const Int8Product& p, cudaStream_t s) {
+    const int64_t bx = (p.n + kGT - 1) / kGT, by = (p.m + kGT - 1) / kGT;
+    if (by > 65535 || bx > INT32_MAX) return cudaErrorInvalidConfiguration;
+    linear_int8_generic_kernel<<<dim3((unsigned)bx, (unsigned)by), 256, 0, s>>>(p);
+    return cudaGetLastError();
+}
+
+int i8_fail(int code, const char* what) { return set_error(code, "%s", what); }
+
+bool known_type(int t) { return t == CLQ_X_F32 || t == CLQ_X_BF16 || t == CLQ_X_F16; }
+
+int check_codes(const char* what, int64_t m, int64_t k, int64_t ld) {
+    if (m < 0 || k < 0) return set_error(CLQ_ERR_SHAPE, "%s: negative shape (%lld %lld)", what, (long long)m, (long long)k);
+    if (ld < k && m > 1)
+        return set_error(CLQ_ERR_SHAPE, "%s: row stride %lld below the row length %lld", what, (long long)ld, (long long)k);
+    return CLQ_OK;
+}
+
+int run_quantize(const QuantRows& q, void* stream) {
+    int dev = 0, rc;
+    if (q.m == 0) return CLQ_OK;
+    if (q.k > 0 && (!q.x || !q.codes)) return i8_fail(CLQ_ERR_ARGUMENT, "null rows or codes");
+    if (!q.scales) return i8_fail(CLQ_ERR_ARGUMENT, "null scales");
+    if ((rc = sm100_device(&dev))) return rc;
+    const cudaError_t e = launch_quantize_rows(q, (cudaStream_t)stream);
+    return e == cudaSuccess ? CLQ_OK : set_error(CLQ_ERR_CUDA, "row quantization: %s", cudaGetErrorString(e));
+}
+
+}  // namespace
+
+cudaError_t launch_linear_int8(const Int8Product& p, cudaStream_t s) { return launch_linear_int8_generic(p, s); }
+
+}  // namespace clq
+
+// ---------------------------------------------------------------------------
+
+using clq::i8_fail;
+
+extern "C" {
+
+int clq_quantize_rows_device(const void* x, int xtype, int64_t m, int64_t k, int64_t ldx, int8_t* codes, int64_t ldc,
+                             float* scales, void* stream) {
+    return clq_norm_quantize_device(x, xtype, m, k, ldx, nullptr, 0.f, nullptr, xtype, 0, nullptr, 0, codes, ldc, scales,
+                                    stream);
+}
+
+int clq_norm_quantize_device(const void* x, int xtype, int64_t m, int64_t k, int64_t ldx, const float* norm_weight,
+                             float norm_epsilon, const void* residual, int rtype, int64_t ldr, void* residual_out,
+                             int64_t ldro, int8_t* codes, int64_t ldc, float* scales, void* stream) {
+    int rc;
+    if (!clq::known_type(xtype)) return clq::set_error(CLQ_ERR_ARGUMENT, "unknown row type %d", xtype);
+    if (residual && rtype != xtype && rtype != CLQ_X_F32)
+        return clq::set_error(CLQ_ERR_ARGUMENT, "residual type %d beside rows of type %d (the same, or f32)", rtype, xtype);
+    if (residual_out && !residual) return i8_fail(CLQ_ERR_ARGUMENT, "a residual output without a residual");
+    if ((rc = clq::check_codes("codes", m, k, ldc))) return rc;
+    if (ldx < 0 || (residual && ldr < 0)) return i8_fail(CLQ_ERR_SHAPE, "negative row stride");
+    if (residual_out && m > 1 && ldro < k)
+        return clq::set_error(CLQ_ERR_SHAPE, "residual output stride %lld below the row length %lld", (long long)ldro,
+                              (long long)k);
+    if (norm_weight && !(norm_epsilon >= 0.f)) return i8_fail(CLQ_ERR_ARGUMENT, "the norm's epsilon must not be negative");
+    clq::QuantRows q = {};
+    q.x = x;
+    q.xtype = xtype;
+    q.m = m;
+    q.k = k;
+    q.ldx = ldx;
+    q.norm_w = norm_weight;
+    q.eps = norm_epsilon;
+    q.res = residual;
+    q.rtype = rtype;
+    q.ldr = ldr;
+    q.res_out = residual_out;
+    q.ldro = ldro;
+    q.codes = codes;
+    q.ldc = ldc;
+    q.scales = scales;
+    return clq::run_quantize(q, stream);
+}
+
+int clq_swiglu_quantize_device(const void* gate, int64_t ldg, const void* up, int64_t ldu, int xtype, int64_t m, int64_t k,
+                               int8_t* codes, int64_t ldc, float* scales, void* stream) {
+    int rc;
+    if (!clq::known_type(xtype)) return clq::set_error(CLQ_ERR_ARGUMENT, "unknown row type %d", xtype);
+    if ((rc = clq::check_codes("codes", m, k, ldc))) return rc;
+    if (ldg < 0 || ldu < 0) return i8_fail(CLQ_ERR_SHAPE, "negative row stride");
+    if (!gate && m > 0 && k > 0) return i8_fail(CLQ_ERR_ARGUMENT, "null gate");
+    clq::QuantRows q = {};
+    q.x = up;
+    q.xtype = xtype;
+    q.m = m;
+    q.k = k;
+    q.ldx = ldu;
+    q.gate = gate;
+    q.ldg = ldg;
+    q.rtype = xtype;
+    q.codes = codes;
+    q.ldc = ldc;
+    q.scales = scales;
+    return clq::run_quantize(q, stream);
+}
+
+int clq_dequantize_rows_device(const int8_t* codes, int64_t ldc, const float* scales, int64_t m, int64_t k, void* out,
+                               int otype, int64_t ldo, void* stream) {
+    int rc, dev = 0;
+    if (!clq::known_type(otype)) return clq::set_error(CLQ_ERR_ARGUMENT, "unknown output type %d", otype);
+    if ((rc = clq::check_codes("codes", m, k, ldc))) return rc;
+    if ((rc = clq::check_codes("values", m, k, ldo))) return rc;
+    if (m == 0 || k == 0) return CLQ_OK;
+    if (!codes || !scales || !out) return i8_fail(CLQ_ERR_ARGUMENT, "null codes, scales or output");
+    if ((rc = clq::sm100_device(&dev))) return rc;
+    const cudaError_t e = clq::launch_dequantize_rows(codes, ldc, scales, m, k, out, otype, ldo, (cudaStream_t)stream);
+    return e == cudaSuccess ? CLQ_OK : clq::set_error(CLQ_ERR_CUDA, "row dequantization: %s", cudaGetErrorString(e));
+}
+
+int clq_linear_int8_device(const int8_t* x, int64_t ldx, const float* x_scales, int64_t m, const int8_t* w, int64_t ldw,
+                           const float* w_scales, int64_t n, int64_t k, const float* residual, int64_t ldr, void* out,
+                           int otype, int64_t ldo, void* stream) {
+    int rc, dev = 0;
+    if (!clq::known_type(otype)) return clq::set_error(CLQ_ERR_ARGUMENT, "unknown output type %d", otype);
+    if ((rc = clq::check_codes("activation codes", m, k, ldx))) return rc;
+    if ((rc = clq::check_codes("weight codes", n, k, ldw))) return rc;
+    if (k > CLQ_INT8_MAX_K)
+        return clq::set_error(CLQ_ERR_UNSUPPORTED, "rows of %lld codes (32-bit sums hold %d)", (long long)k, CLQ_INT8_MAX_K);
+    if (m > 1 && (ldo < n || (residual && ldr < n)))
+        return clq::set_error(CLQ_ERR_SHAPE, "output or residual stride below %lld columns", (long long)n);
+    if (m == 0 || n == 0) return CLQ_OK;
+    if (!out || !x_scales || !w_scales || (k > 0 && (!x || !w))) return i8_fail(CLQ_ERR_ARGUMENT, "null operand or output");
+    if ((rc = clq::sm100_device(&dev))) return rc;
+    clq::Int8Product p = {};
+    p.x = x;
+    p.ldx = ldx;
+    p.xs = x_scales;
+    p.m = m;
+    p.w = w;
+    p.ldw = ldw;
+    p.ws = w_scales;
+    p.n = n;
+    p.k = k;
+    p.res = residual;
+    p.ldr = ldr;
+    p.out = out;
+    p.otype = otype;
+    p.ldo = ldo;
+    const cudaError_t e = clq::launch_linear_int8(p, (cudaStream_t)stream);
+    return e == cudaSuccess ? CLQ_OK : clq::set_error(CLQ_ERR_CUDA, "8-bit linear: %s", cudaGetErrorString(e));
+}
+
+}  // extern "C"

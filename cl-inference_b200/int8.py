@@ -1,0 +1,263 @@
+"""8-bit rows and their product (clq_quantize_rows_device, clq_norm_quantize_device,
+clq_swiglu_quantize_device, clq_dequantize_rows_device, clq_linear_int8_device).
+
+An Int8Rows holds rows of int8 codes with one f32 scale a row: the tokens of an
+activation, or the output channels of a weight.  The steps of a decoder layer
+(local/blocks.lisp:327-392) in 8-bit activations:
+
+  wq = quantize_rows(w)                       once: a weight [n, k], or store.dequantize()
+  q, h = norm_quantize(y, norm_w, eps, residual=h)   residual add + RMSNorm + rounding
+  gate_up = linear_int8(q, wq)                [m, 2 f], f32 / bf16 / f16
+  q = swiglu_quantize(gate_up[:, :f], gate_up[:, f:])
+  y = linear_int8(q, w_down)
+
+Tensors are on the current CUDA device, rows with a unit last stride (others
+are copied) and any row stride.  Work is queued on the current stream, or on
+STREAM (a cudaStream_t handle): outputs then belong to that stream.
+"""
+from . import _lib
+from .store import _XTYPE
+
+_lib_quantize = _lib.lib.clq_norm_quantize_device
+_lib_swiglu = _lib.lib.clq_swiglu_quantize_device
+_lib_dequantize = _lib.lib.clq_dequantize_rows_device
+_lib_linear = _lib.lib.clq_linear_int8_device
+
+_types = None  # torch dtype -> clq_xtype
+
+
+def _torch():
+    global _types
+    import torch
+    if _types is None:
+        _types = {getattr(torch, name): code for name, code in _XTYPE.items()}
+    return torch
+
+
+def _type_code(torch, dtype, what):
+    code = _types.get(dtype)
+    if code is None:
+        raise ValueError(f"{what}: float32, bfloat16 or float16, not {dtype}")
+    return code
+
+
+def _matrix(torch, t, what, shape=None):
+    """T as a CUDA matrix on the current device with unit last stride."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dim() != 2:
+        raise ValueError(f"{what}: a CUDA matrix")
+    if shape is not None and t.shape != shape:
+        raise ValueError(f"{what} is {tuple(t.shape)}, {tuple(shape)} is wanted")
+    if t.get_device() != torch.cuda.current_device():
+        raise ValueError(f"{what} lives on device {t.get_device()}, current device is {torch.cuda.current_device()}")
+    return t if t.stride(1) == 1 or t.shape[1] <= 1 else t.contiguous()
+
+
+def _vector(torch, t, n, what):
+    if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype != torch.float32 or t.dim() != 1 or t.shape[0] != n:
+        raise ValueError(f"{what}: a CUDA float32 vector of {n}")
+    if t.get_device() != torch.cuda.current_device():
+        raise ValueError(f"{what} lives on device {t.get_device()}, current device is {torch.cuda.current_device()}")
+    return t if n <= 1 or t.stride(0) == 1 else t.contiguous()
+
+
+def _writable(torch, t, what, shape, dtype):
+    """T as an output: nothing may be copied, and its rows must not share memory."""
+    if (not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype != dtype or t.shape != shape
+            or t.get_device() != torch.cuda.current_device() or (shape[1] > 1 and t.stride(1) != 1)
+            or (shape[0] > 1 and t.stride(0) < shape[1])):
+        raise ValueError(f"{what}: a {dtype} matrix {tuple(shape)} on the current device, rows apart with unit last stride")
+    return t
+
+
+def _ld(t):
+    """Row stride of a matrix; a single row has none to speak of."""
+    return t.stride(0) if t.shape[0] > 1 else (t.shape[1] + 15) // 16 * 16
+
+
+def _on(torch, stream, tensors, call):
+    """CALL() with STREAM (a handle) as the current stream, so that what it
+    allocates belongs to that stream; TENSORS are kept until STREAM is done."""
+    side = torch.cuda.ExternalStream(stream)
+    for t in tensors:
+        if t is not None:
+            t.record_stream(side)
+    with torch.cuda.stream(side):
+        return call()
+
+
+class Int8Rows:
+    """CODES int8 [m, k] (any row stride, unit last stride) and SCALES f32 [m]."""
+
+    __slots__ = ("codes", "scales")
+
+    def __init__(self, codes, scales):
+        torch = _torch()
+        codes = _matrix(torch, codes, "codes")
+        if codes.dtype != torch.int8:
+            raise ValueError(f"codes: int8, not {codes.dtype}")
+        self.codes, self.scales = codes, _vector(torch, scales, codes.shape[0], "scales")
+
+    @property
+    def shape(self):
+        return self.codes.shape
+
+    def __len__(self):
+        return self.codes.shape[0]
+
+    def __getitem__(self, rows):
+        """Rows by a slice with step 1, sharing the memory (a row range of a weight)."""
+        if not isinstance(rows, slice) or rows.step not in (None, 1):
+            raise TypeError("Int8Rows takes slices of rows")
+        return Int8Rows(self.codes[rows], self.scales[rows])
+
+    def dequantize(self, dtype=None, out=None, stream=None):
+        """codes * scales in DTYPE (float32 without one), into OUT when given."""
+        torch = _torch()
+        if stream is not None:
+            return _on(torch, stream, (self.codes, self.scales, out), lambda: self.dequantize(dtype, out))
+        m, k = self.codes.shape
+        if dtype is None:
+            dtype = torch.float32 if out is None else out.dtype
+        code = _type_code(torch, dtype, "dtype")
+        if out is None:
+            out = torch.empty((m, k), dtype=dtype, device=self.codes.device)
+        else:
+            _writable(torch, out, "out", (m, k), dtype)
+        _lib.check(_lib_dequantize(self.codes.data_ptr(), _ld(self.codes), self.scales.data_ptr(), m, k, out.data_ptr(),
+                                   code, _ld(out), torch.cuda.current_stream().cuda_stream))
+        return out
+
+
+def _empty_rows(torch, m, k, device):
+    """Uninitialised Int8Rows whose code rows start on 16-byte boundaries."""
+    q = Int8Rows.__new__(Int8Rows)
+    pitch = (k + 15) // 16 * 16
+    codes = torch.empty((m, pitch), dtype=torch.int8, device=device)
+    q.codes = codes if pitch == k else codes[:, :k]
+    q.scales = torch.empty(m, dtype=torch.float32, device=device)
+    return q
+
+
+def quantize_rows(x, stream=None):
+    """The Int8Rows of X [m, k] (float32, bfloat16 or float16)."""
+    return norm_quantize(x, stream=stream)
+
+
+def norm_quantize(x, norm_weight=None, eps=1e-5, residual=None, residual_out=None, stream=None):
+    """The Int8Rows of RMSNorm(x + residual) * norm_weight, in one pass over the rows.
+
+    Without NORM_WEIGHT (f32 [k]) the sum itself is coded; without RESIDUAL (x's
+    type, or f32) x alone.  With a residual returns (rows, x + residual), the sum
+    in the residual's type: RESIDUAL_OUT, which may be RESIDUAL, or a new tensor.
+    """
+    torch = _torch()
+    if stream is not None:
+        return _on(torch, stream, (x, norm_weight, residual, residual_out),
+                   lambda: norm_quantize(x, norm_weight, eps, residual, residual_out))
+    x = _matrix(torch, x, "x")
+    m, k = x.shape
+    xtype = _type_code(torch, x.dtype, "x")
+    wptr = rptr = optr = None
+    rtype, ldr, ldo = xtype, 0, 0
+    if norm_weight is not None:
+        norm_weight = _vector(torch, norm_weight, k, "norm_weight")
+        wptr = norm_weight.data_ptr()
+    if residual is not None:
+        given, residual = residual, _matrix(torch, residual, "residual", x.shape)
+        rtype = _type_code(torch, residual.dtype, "residual")
+        if rtype not in (xtype, _lib.CLQ_X_F32):
+            raise ValueError(f"residual: {x.dtype} or float32, not {residual.dtype}")
+        if residual_out is None:
+            residual_out = torch.empty((m, k), dtype=residual.dtype, device=x.device)
+        else:
+            _writable(torch, residual_out, "residual_out", (m, k), residual.dtype)
+            _apart(residual_out, given, "residual_out")
+            _apart(residual_out, x, "residual_out")
+        rptr, ldr, optr, ldo = residual.data_ptr(), _ld(residual), residual_out.data_ptr(), _ld(residual_out)
+    elif residual_out is not None:
+        raise ValueError("residual_out needs a residual")
+    q = _empty_rows(torch, m, k, x.device)
+    _lib.check(_lib_quantize(x.data_ptr(), xtype, m, k, _ld(x), wptr, eps, rptr, rtype, ldr, optr, ldo,
+                             q.codes.data_ptr(), _ld(q.codes), q.scales.data_ptr(),
+                             torch.cuda.current_stream().cuda_stream))
+    return q if residual is None else (q, residual_out)
+
+
+def swiglu_quantize(gate, up, stream=None):
+    """The Int8Rows of silu(gate) * up, both [m, k] of one type (two halves of one product, say)."""
+    torch = _torch()
+    if stream is not None:
+        return _on(torch, stream, (gate, up), lambda: swiglu_quantize(gate, up))
+    gate, up = _matrix(torch, gate, "gate"), _matrix(torch, up, "up", gate.shape)
+    if gate.dtype != up.dtype:
+        raise ValueError(f"gate is {gate.dtype}, up is {up.dtype}")
+    xtype = _type_code(torch, gate.dtype, "gate")
+    m, k = gate.shape
+    q = _empty_rows(torch, m, k, gate.device)
+    _lib.check(_lib_swiglu(gate.data_ptr(), _ld(gate), up.data_ptr(), _ld(up), xtype, m, k, q.codes.data_ptr(),
+                           _ld(q.codes), q.scales.data_ptr(), torch.cuda.current_stream().cuda_stream))
+    return q
+
+
+def linear_int8(x, w, out=None, dtype=None, residual=None, stream=None):
+    """out[m, n] = X [m, k] . W [n, k]^T of two Int8Rows, plus an optional f32
+    RESIDUAL [m, n] (which may be OUT), rounded once to DTYPE (OUT's, or float32).
+    The products are summed in 32-bit integers: exact, for k up to 131071."""
+    torch = _torch()
+    if not isinstance(x, Int8Rows) or not isinstance(w, Int8Rows):
+        raise ValueError("linear_int8 multiplies Int8Rows")
+    if stream is not None:
+        return _on(torch, stream, (x.codes, x.scales, w.codes, w.scales, out, residual),
+                   lambda: linear_int8(x, w, out, dtype, residual))
+    m, k = x.codes.shape
+    n = w.codes.shape[0]
+    if w.codes.shape[1] != k:
+        raise ValueError(f"rows of {k} codes against a weight of {tuple(w.codes.shape)}")
+    device = x.codes.get_device()
+    if device != w.codes.get_device() or device != torch.cuda.current_device():
+        raise ValueError(f"x on device {device}, w on {w.codes.get_device()}, current device is "
+                         f"{torch.cuda.current_device()}")
+    if dtype is None:
+        dtype = torch.float32 if out is None else out.dtype
+    code = _type_code(torch, dtype, "dtype")
+    if out is None:
+        out = torch.empty((m, n), dtype=dtype, device=x.codes.device)
+    else:
+        _writable(torch, out, "out", (m, n), dtype)
+    rptr, ldr = None, 0
+    if residual is not None:
+        if residual.dtype != torch.float32:
+            raise ValueError(f"residual: float32, not {residual.dtype}")
+        given, residual = residual, _matrix(torch, residual, "residual", (m, n))
+        _apart(out, given, "out")
+        rptr, ldr = residual.data_ptr(), _ld(residual)
+    _lib.check(_lib_linear(x.codes.data_ptr(), _ld(x.codes), x.scales.data_ptr(), m, w.codes.data_ptr(), _ld(w.codes),
+                           w.scales.data_ptr(), n, k, rptr, ldr, out.data_ptr(), code, _ld(out),
+                           torch.cuda.current_stream().cuda_stream))
+    return out
+
+
+def _span(t):
+    """First byte and the byte after the last of a matrix."""
+    a = t.data_ptr()
+    reach = sum((n - 1) * s for n, s in zip(t.shape, t.stride())) if t.numel() else -1
+    return a, a + (reach + 1) * t.element_size()
+
+
+def _overlap(a, b):
+    """Whether two matrices of unit last stride share memory."""
+    (a0, a1), (b0, b1) = _span(a), _span(b)
+    if a0 >= b1 or b0 >= a1:
+        return False
+    pitch = a.stride(0) * a.element_size()
+    if pitch > 0 and pitch == b.stride(0) * b.element_size():  # columns of one buffer, side by side
+        at = (b0 - a0) % pitch
+        return at < a.shape[1] * a.element_size() or at + b.shape[1] * b.element_size() > pitch
+    return True
+
+
+def _apart(out, given, what):
+    """Refuses an output that shares memory with an input other than by being it."""
+    if out is not given and _overlap(out, given) and not (
+            out.data_ptr() == given.data_ptr() and out.stride() == given.stride() and out.dtype == given.dtype):
+        raise ValueError(f"{what}: the input itself, or memory apart from it")

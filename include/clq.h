@@ -336,6 +336,45 @@ int clq_rope_device(float *x, int64_t count, int heads, int head_dim, int64_t po
 int clq_attend_device(const float *q, int64_t count, int n_heads, int64_t q_pos_stride, const clq_kv_cache *cache,
                       int layer, int64_t end, int64_t query_start, float *out, int64_t ldo, void *stream);
 
+/* ---- 8-bit activations ------------------------------------------------------
+ * No counterpart in the reference (its activations are f32).  Rows of int8
+ * codes with one f32 scale a row, value = code * scale, made with the rule of
+ * the Q8 cache codec over the whole row: step = max(FLT_MIN, peak / 127), code =
+ * clamp(round-half-even(v / step), -127, 127), the quotient formed as a product
+ * with the rounded 1 / step; an all-zero row has the scale 1, and a row with a
+ * non-finite value has codes 0 and the scale NaN.  Row strides are in elements;
+ * each row is contiguous.  Any alignment is taken; code rows that start on
+ * 16-byte boundaries (base and stride) run on the fast kernels.  All calls are
+ * asynchronous on STREAM, allocate nothing and keep nothing.
+ */
+/* M rows of K elements of XTYPE (clq_xtype). */
+int clq_quantize_rows_device(const void *x, int xtype, int64_t m, int64_t k, int64_t ldx, int8_t *codes,
+                             int64_t ldc, float *scales, void *stream);
+/* h = x + residual, rounded into RESIDUAL_OUT; the codes are those of the f32
+ * h * norm_weight and the scales those times 1 / sqrt(mean(h^2) + norm_epsilon)
+ * (the residual addition of layer-forward, local/blocks.lisp:387-392, and the
+ * apply-rmsnorm of the next block, :115-116).  RESIDUAL, RESIDUAL_OUT (which may
+ * be RESIDUAL) and NORM_WEIGHT (f32 [K]; without it h itself is coded) may be
+ * null.  RTYPE, of both residuals, is XTYPE or CLQ_X_F32.  A row whose sum of
+ * squares leaves f32 counts as non-finite. */
+int clq_norm_quantize_device(const void *x, int xtype, int64_t m, int64_t k, int64_t ldx, const float *norm_weight,
+                             float norm_epsilon, const void *residual, int rtype, int64_t ldr, void *residual_out,
+                             int64_t ldro, int8_t *codes, int64_t ldc, float *scales, void *stream);
+/* The codes of silu(gate) * up (local/blocks.lisp:151-154). */
+int clq_swiglu_quantize_device(const void *gate, int64_t ldg, const void *up, int64_t ldu, int xtype, int64_t m,
+                               int64_t k, int8_t *codes, int64_t ldc, float *scales, void *stream);
+/* out[i, c] = codes[i, c] * scales[i], rounded to OTYPE (clq_xtype). */
+int clq_dequantize_rows_device(const int8_t *codes, int64_t ldc, const float *scales, int64_t m, int64_t k,
+                               void *out, int otype, int64_t ldo, void *stream);
+/* out[t, j] = sum_c x[t, c] w[j, c] * w_scales[j] * x_scales[t] (+ residual[t, j]) for
+ * M token rows and N channel rows of K codes (any int8 value), rounded once to OTYPE: the
+ * linear of local/blocks.lisp:106-113 with both operands in 8 bits.  The sum is an
+ * exact 32-bit integer, which bounds K.  RESIDUAL (f32) may be null, or OUT itself. */
+#define CLQ_INT8_MAX_K 131071
+int clq_linear_int8_device(const int8_t *x, int64_t ldx, const float *x_scales, int64_t m, const int8_t *w,
+                           int64_t ldw, const float *w_scales, int64_t n, int64_t k, const float *residual,
+                           int64_t ldr, void *out, int otype, int64_t ldo, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
