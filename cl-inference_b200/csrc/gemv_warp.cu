@@ -858,6 +858,19 @@ bool encode_rows(CUtensorMap* map, const void* base, int64_t rows, int64_t row_b
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+bool encode_swizzled_rows(CUtensorMap* map, const void* base, int64_t rows, int64_t row_bytes, int64_t stride, int box_rows) {
+    PFN_cuTensorMapEncodeTiled_v12000 fn = encode_tiled();
+    if (!fn || (uintptr_t)base % 16 || stride % 16 || rows < 1 || row_bytes < 1 || box_rows < 1 || box_rows > 256)
+        return false;
+    const cuuint64_t dims[2] = {(cuuint64_t)row_bytes, (cuuint64_t)rows};
+    const cuuint64_t strides[1] = {(cuuint64_t)stride};
+    const cuuint32_t boxd[2] = {128u, (cuuint32_t)box_rows};
+    const cuuint32_t estr[2] = {1u, 1u};
+    return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, boxd, estr,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 namespace {
 // The per-warp kernel's map over a weight's q plane (ROWS rows of ROW_BYTES),
 // one box per unit of 16 rows x BOX bytes: Q4_K / Q6_K plain; Q4_0 (128-byte

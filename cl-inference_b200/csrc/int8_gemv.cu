@@ -1,0 +1,140 @@
+// int8_gemv.cu -- the 8-bit product for up to 16 tokens: every weight byte is
+// read once, straight into the registers of an m16n8k32 integer MMA, so the
+// kernel is bound by the weight's bytes (and, below a few MB, by latency).
+//
+// A CTA takes 8 R weight rows; its warps take the 64-byte columns of K in turn
+// and add their integer sums in shared memory at the end.  In one 64-byte
+// column lane (g, q) = (lane / 4, lane % 4) loads the 16 bytes at 16 q of weight
+// row g (eight rows, whole 32-byte sectors) and of token rows g and g + 8.  Words 0
+// and 1 of the load are the B (and A) fragments of one MMA, words 2 and 3 those
+// of a second: the two operands permute K alike, which a sum does not see.
+#include <cstdint>
+
+#include <cuda_runtime.h>
+
+#include "../../include/clq.h"
+#include "clq_internal.h"
+#include "int8_out.cuh"
+#include "launch.cuh"
+#include "pipeline.cuh"
+
+namespace clq {
+namespace {
+
+constexpr int kGvWarps = 8;
+
+__device__ __forceinline__ void mma_s8(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                       uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// Bytes [k0, k0 + 16) of a row of K codes, zeros past its end.
+__device__ __forceinline__ uint4 load_tail(const int8_t* row, int64_t k0, int64_t k) {
+    if (k0 + 16 <= k) return *reinterpret_cast<const uint4*>(row + k0);
+    uint32_t w[4] = {0, 0, 0, 0};
+    for (int i = 0; k0 + i < k; i++) w[i >> 2] |= (uint32_t)(uint8_t)row[k0 + i] << (8 * (i & 3));
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// HI: tokens 8..15 are present.  U: 64-byte columns a warp has in flight.
+template <typename OT, int R, bool HI, int U>
+__global__ void __launch_bounds__(kGvWarps * 32) int8_gemv_kernel(const Int8Product P) {
+    __shared__ int part[kGvWarps][R][HI ? 4 : 2][32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, q = lane & 3;
+    const int64_t n0 = (int64_t)blockIdx.x * 8 * R;
+    pipe::grid_dependency_wait();
+    pipe::allow_dependents();
+
+    const int8_t* wr[R];
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+        const int64_t n = n0 + 8 * r + g;
+        wr[r] = P.w + (n < P.n ? n : P.n - 1) * P.ldw;  // rows past the last repeat it and are not written
+    }
+    const bool lo_in = g < P.m, hi_in = HI && g + 8 < P.m;
+    const int8_t* xlo = P.x + (lo_in ? g : 0) * P.ldx;
+    const int8_t* xhi = P.x + (hi_in ? g + 8 : 0) * P.ldx;
+    int acc[R][4] = {};
+    const uint4 zero = make_uint4(0, 0, 0, 0);
+    auto column = [&](const uint4 (&w)[R], const uint4& a, const uint4& b) {
+#pragma unroll
+        for (int r = 0; r < R; r++) {
+            mma_s8(acc[r], a.x, b.x, a.y, b.y, w[r].x, w[r].y);
+            mma_s8(acc[r], a.z, b.z, a.w, b.w, w[r].z, w[r].w);
+        }
+    };
+    const int64_t whole = P.k / 64;
+    int64_t c = warp;
+    for (; c + (U - 1) * kGvWarps < whole; c += U * kGvWarps) {
+        uint4 w[U][R], a[U], b[U];
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int64_t k0 = (c + u * kGvWarps) * 64 + 16 * q;
+#pragma unroll
+            for (int r = 0; r < R; r++) w[u][r] = __ldcs(reinterpret_cast<const uint4*>(wr[r] + k0));
+            a[u] = lo_in ? *reinterpret_cast<const uint4*>(xlo + k0) : zero;
+            b[u] = hi_in ? *reinterpret_cast<const uint4*>(xhi + k0) : zero;
+        }
+#pragma unroll
+        for (int u = 0; u < U; u++) column(w[u], a[u], b[u]);
+    }
+    for (; c * 64 < P.k; c += kGvWarps) {  // the last columns, one at a time
+        const int64_t k0 = c * 64 + 16 * q;
+        uint4 w[R];
+#pragma unroll
+        for (int r = 0; r < R; r++) w[r] = load_tail(wr[r], k0, P.k);
+        column(w, lo_in ? load_tail(xlo, k0, P.k) : zero, hi_in ? load_tail(xhi, k0, P.k) : zero);
+    }
+#pragma unroll
+    for (int r = 0; r < R; r++)
+#pragma unroll
+        for (int i = 0; i < (HI ? 4 : 2); i++) part[warp][r][i][lane] = acc[r][i];
+    __syncthreads();
+    // output (t, 8 r + j): lane 4 (t % 8) + j / 2, register j % 2 + 2 (t / 8)
+    OT* out = static_cast<OT*>(P.out);
+    for (int e = threadIdx.x; e < (int)P.m * 8 * R; e += kGvWarps * 32) {
+        const int t = e / (8 * R), jn = e % (8 * R), r = jn >> 3, j = jn & 7;
+        const int64_t n = n0 + jn;
+        if (n >= P.n) continue;
+        const int l = 4 * (t & 7) + (j >> 1), i = (j & 1) + (HI ? 2 * (t >> 3) : 0);
+        int sum = 0;
+#pragma unroll
+        for (int w = 0; w < kGvWarps; w++) sum += part[w][r][i][l];
+        float v = int8_scaled(sum, P.ws[n], P.xs[t]);
+        if (P.res) v = __fadd_rn(v, P.res[t * P.ldr + n]);
+        out[t * P.ldo + n] = int8_round<OT>(v);
+    }
+}
+
+template <typename OT, int R, bool HI>
+cudaError_t launch_gv(const Int8Product& p, cudaStream_t s) {
+    const int64_t blocks = (p.n + 8 * R - 1) / (8 * R);
+    if (blocks > INT32_MAX) return cudaErrorNotSupported;
+    return pipe::launch_pdl(int8_gemv_kernel<OT, R, HI, 8 / R>, dim3((unsigned)blocks), kGvWarps * 32, 0, s, p);
+}
+
+template <typename OT>
+cudaError_t launch_gv_type(const Int8Product& p, cudaStream_t s) {
+    const bool hi = p.m > 8;
+    const int64_t sms = sm_count();
+    if (p.n >= 32 * 2 * sms) return hi ? launch_gv<OT, 4, true>(p, s) : launch_gv<OT, 4, false>(p, s);
+    if (p.n >= 16 * sms) return hi ? launch_gv<OT, 2, true>(p, s) : launch_gv<OT, 2, false>(p, s);
+    return hi ? launch_gv<OT, 1, true>(p, s) : launch_gv<OT, 1, false>(p, s);
+}
+
+}  // namespace
+
+cudaError_t launch_int8_gemv(const Int8Product& p, cudaStream_t s) {
+    if (p.m > 16 || !int8_aligned(p)) return cudaErrorNotSupported;
+    switch (p.otype) {
+    case CLQ_X_F32: return launch_gv_type<float>(p, s);
+    case CLQ_X_BF16: return launch_gv_type<__nv_bfloat16>(p, s);
+    case CLQ_X_F16: return launch_gv_type<__half>(p, s);
+    default: return cudaErrorInvalidValue;
+    }
+}
+
+}  // namespace clq

@@ -91,7 +91,15 @@ int run_quantize(const QuantRows& q, void* stream) {
 
 }  // namespace
 
-cudaError_t launch_linear_int8(const Int8Product& p, cudaStream_t s) { return launch_linear_int8_generic(p, s); }
+bool int8_aligned(const Int8Product& p) {
+    return !(((uintptr_t)p.x | (uintptr_t)p.w | (uint64_t)p.ldx | (uint64_t)p.ldw) & 15);
+}
+
+cudaError_t launch_linear_int8(const Int8Product& p, cudaStream_t s) {
+    if (p.k < 1 || !int8_aligned(p)) return launch_linear_int8_generic(p, s);
+    cudaError_t e = p.m <= 16 ? launch_int8_gemv(p, s) : launch_int8_gemm(p, s);
+    return e == cudaErrorNotSupported ? launch_linear_int8_generic(p, s) : e;
+}
 
 }  // namespace clq
 
