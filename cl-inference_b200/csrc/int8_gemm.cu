@@ -19,6 +19,7 @@
 // the library's device status word, stops issuing, drains what it issued and
 // frees its tensor memory.
 #include <algorithm>
+#include <atomic>
 #include <cstdint>
 
 #include <cuda.h>
@@ -66,8 +67,13 @@ __device__ __forceinline__ uint32_t map_rank(uint32_t addr, uint32_t rank) {
     asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(addr), "r"(rank));
     return a;
 }
-__device__ __forceinline__ void store_cluster(uint32_t addr, int v) {
-    asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
+__device__ __forceinline__ int4 load_cluster(uint32_t addr) {
+    int4 v;
+    asm volatile("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                 : "r"(addr)
+                 : "memory");
+    return v;
 }
 __device__ __forceinline__ void arrive_cluster(uint32_t bar) {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
@@ -141,6 +147,9 @@ __device__ __forceinline__ void tmem_load32(uint32_t addr, int (&v)[32]) {
         : "r"(addr));
     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
+__device__ __forceinline__ void prefetch_map(const void* map) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
+}
 // A box of MAP at (X bytes, row Y) into this CTA's DST, counted on BAR, a
 // shared::cluster address that may lie in the pair's other CTA.
 __device__ __forceinline__ void tensor_copy_pair(void* dst, const void* map, int x, int y, uint32_t bar) {
@@ -150,63 +159,161 @@ __device__ __forceinline__ void tensor_copy_pair(void* dst, const void* map, int
         "l"(map), "r"(x), "r"(y), "r"(bar)
         : "memory");
 }
-// Bounded wait that spins without sleeping (a stage is a few hundred cycles).
+// One lane of a converged warp.  The copying and the issuing warp run their
+// loops as whole warps and elect a lane around the asynchronous instructions
+// alone: where a branch on the lane enclosed the loop, a tcgen05.commit after
+// four MMAs cost about 800 cycles (0.30 us a stage whatever the tile; 256
+// x 256 tiles took 0.41, and their MMAs alone need 0.28).
+__device__ __forceinline__ bool elect_one() {
+    uint32_t e;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(e));
+    return e != 0;
+}
+// Bounded wait of a whole warp that spins without sleeping (a stage is a few
+// hundred cycles); every lane gets the same answer.
 __device__ __forceinline__ bool wait_spin(uint64_t* bar, uint32_t parity, int* err) {
-    for (uint32_t i = 0; i < kWaitLimit; i++) {
-        if (mbar_test(bar, parity)) return true;
-        if ((i & 1023) == 1023 && *(volatile int*)err) return false;
+    bool ok = false;
+    uint32_t i = 0;
+    for (; i < kWaitLimit; i++) {
+        if ((ok = mbar_test(bar, parity))) break;
+        if ((i & 1023) == 1023 && *(volatile int*)err) break;
     }
-    atomicExch(err, CLQ_ERR_TIMEOUT);
-    return false;
+    if (i == kWaitLimit) atomicExch(err, CLQ_ERR_TIMEOUT);
+    return __all_sync(0xffffffffu, ok);
 }
 __device__ __forceinline__ uint8_t* align1024(uint8_t* p) {
     return reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(p) + 1023) & ~(uintptr_t)1023);
 }
 
-// Outputs of weight row N (one per lane) for the 32 tokens T0.. from their sums.
-template <typename OT>
-__device__ __forceinline__ void emit32(const Int8Product& p, const int (&v)[32], int64_t n, float wsn, int64_t t0, int lane) {
-    const float xs_lane = t0 + lane < p.m ? p.xs[t0 + lane] : 0.f;
-    const bool in = n < p.n;
-    const int cnt = p.m - t0 < 32 ? (int)(p.m - t0) : 32;
-    OT* out = static_cast<OT*>(p.out) + t0 * p.ldo + n;
-    const float* res = p.res ? p.res + t0 * p.ldr + n : nullptr;
-    float r[32];
-    if (res) {  // the residual's loads in flight before any is used
+// Outputs of weight row N (one per lane) for CNT <= 32 tokens from T0 on, from
+// their sums; X: the scale of token T0 + lane.  Each loop is one straight run of
+// independent instructions, and the pointers step by a row: with a test for the
+// residual inside a single loop, or the product j * ldo for an address, 256
+// columns took 9.0 us instead of 2.9.
+template <typename OT, bool RES>
+__device__ __forceinline__ void emit_columns(const Int8Product& p, const int (&v)[32], int64_t n, float wsn, int64_t t0,
+                                             int cnt, float x) {
+    if (n >= p.n) cnt = 0;
+    float o[32];
+    if constexpr (RES) {  // the residual's loads in flight before any is used
+        const float* res = p.res + t0 * p.ldr + n;
 #pragma unroll
-        for (int j = 0; j < 32; j++) r[j] = in && j < cnt ? res[j * p.ldr] : 0.f;
+        for (int j = 0; j < 32; j++, res += p.ldr) o[j] = j < cnt ? *res : 0.f;
     }
 #pragma unroll
     for (int j = 0; j < 32; j++) {
-        float o = int8_scaled(v[j], wsn, __shfl_sync(0xffffffffu, xs_lane, j));
-        if (res) o = __fadd_rn(o, r[j]);
-        if (in && j < cnt) out[j * p.ldo] = int8_round<OT>(o);
+        const float y = int8_scaled(v[j], wsn, __shfl_sync(0xffffffffu, x, j));
+        if constexpr (RES) o[j] = __fadd_rn(y, o[j]);
+        else o[j] = y;
+    }
+    OT* out = static_cast<OT*>(p.out) + t0 * p.ldo + n;
+#pragma unroll
+    for (int j = 0; j < 32; j++, out += p.ldo)
+        if (j < cnt) *out = int8_round<OT>(o[j]);
+}
+template <typename OT>
+__device__ __forceinline__ void emit32(const Int8Product& p, const int (&v)[32], int64_t n, float wsn, int64_t t0, int cnt,
+                                       float x) {
+    __syncwarp();
+    if (p.res) emit_columns<OT, true>(p, v, n, wsn, t0, cnt, x);
+    else emit_columns<OT, false>(p, v, n, wsn, t0, cnt, x);
+}
+
+// Four neighbouring outputs O of one token: one store where OUT allows it.
+template <typename OT>
+__device__ __forceinline__ void store4(OT* out, const float (&o)[4], int cnt) {
+    if (cnt >= 4 && reinterpret_cast<uintptr_t>(out) % (4 * sizeof(OT)) == 0) {
+        OT h[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) h[i] = int8_round<OT>(o[i]);
+        if constexpr (sizeof(OT) == 4) *reinterpret_cast<uint4*>(out) = *reinterpret_cast<const uint4*>(h);
+        else *reinterpret_cast<uint2*>(out) = *reinterpret_cast<const uint2*>(h);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            if (i < cnt) out[i] = int8_round<OT>(o[i]);
+    }
+}
+
+// Tokens T0, T0 + 4, .. (B of them) of rows N..N + 3, CNT of which exist: the
+// SPLITS parts' sums at AT (this CTA's address of token T0's, a token 4 * kRows * 4
+// bytes after the last) added up and written.  Two parts' loads are in flight
+// together.
+template <typename OT, int B, bool RES>
+__device__ __forceinline__ void join_parts(const Int8Product& P, uint32_t at, int splits, int64_t t0, int64_t n, int cnt,
+                                           const float (&wsn)[4], const float* xs) {
+    float4 r[B] = {};
+    if constexpr (RES) {
+        const float* res = P.res + t0 * P.ldr + n;
+#pragma unroll
+        for (int b = 0; b < B; b++, res += 4 * P.ldr) {
+            if (cnt > 0) r[b].x = res[0];
+            if (cnt > 1) r[b].y = res[1];
+            if (cnt > 2) r[b].z = res[2];
+            if (cnt > 3) r[b].w = res[3];
+        }
+    }
+    int4 a[B] = {};
+    for (int q = 0; q < splits; q += 2) {
+        const int once = q + 1 < splits ? -1 : 0;  // an odd last part is read twice and counted once
+        const uint32_t one = map_rank(at, (uint32_t)q), two = map_rank(at, (uint32_t)(q - once));
+        int4 v[B], v2[B];
+#pragma unroll
+        for (int b = 0; b < B; b++) {
+            v[b] = load_cluster(one + b * 4 * kRows * 4);
+            v2[b] = load_cluster(two + b * 4 * kRows * 4);
+        }
+#pragma unroll
+        for (int b = 0; b < B; b++) {
+            a[b].x += v[b].x + (v2[b].x & once);
+            a[b].y += v[b].y + (v2[b].y & once);
+            a[b].z += v[b].z + (v2[b].z & once);
+            a[b].w += v[b].w + (v2[b].w & once);
+        }
+    }
+    OT* out = static_cast<OT*>(P.out) + t0 * P.ldo + n;
+#pragma unroll
+    for (int b = 0; b < B; b++, out += 4 * P.ldo) {
+        const float x = xs[4 * b];
+        float o[4] = {int8_scaled(a[b].x, wsn[0], x), int8_scaled(a[b].y, wsn[1], x), int8_scaled(a[b].z, wsn[2], x),
+                      int8_scaled(a[b].w, wsn[3], x)};
+        if constexpr (RES) {
+            o[0] = __fadd_rn(o[0], r[b].x);
+            o[1] = __fadd_rn(o[1], r[b].y);
+            o[2] = __fadd_rn(o[2], r[b].z);
+            o[3] = __fadd_rn(o[3], r[b].w);
+        }
+        store4<OT>(out, o, cnt);
     }
 }
 
 // ---- tile kernel --------------------------------------------------------------
 
-constexpr int tile_stages(int tn) { return tn == 256 ? 4 : tn == 128 ? 5 : tn == 64 ? 8 : 9; }
-size_t tile_smem(int tn, int splits) {
-    return 1024 + (size_t)tile_stages(tn) * (kABytes + (size_t)tn * kKB) + (splits > 1 ? (size_t)tn * kRows * 4 : 0) +
-           (2 * tile_stages(tn) + 1) * 8 + 16;
+constexpr int tile_stages(int tn) { return tn == 256 ? 4 : tn == 128 ? 6 : tn == 64 ? 8 : 10; }
+constexpr size_t tile_smem(int tn) {
+    return 1024 + (size_t)tile_stages(tn) * (kABytes + (size_t)tn * kKB) + (2 * tile_stages(tn) + 2) * 8 + (size_t)tn * 4;
 }
+static_assert(tile_smem(256) <= kSmemMax && tile_smem(128) <= kSmemMax && tile_smem(64) <= kSmemMax &&
+              tile_smem(32) <= kSmemMax, "shared memory of one SM");
 
 // CTA (blockIdx.x = row tile x SPLITS + part, blockIdx.y = token tile); the
-// SPLITS parts of a tile form a cluster.  Part r of the cluster finishes the
-// tokens [r TN / SPLITS, (r + 1) TN / SPLITS) of the tile.
+// SPLITS parts of a tile form a cluster.  Each part leaves its sums in its own
+// shared memory, over the stages it has done with, as [token][row], and part r
+// finishes the tokens [r TN / SPLITS, (r + 1) TN / SPLITS) from all of them.
 template <typename OT, int TN>
 __global__ void __launch_bounds__(kThreads) int8_tile_kernel(const __grid_constant__ GemmI8 G, int splits) {
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     constexpr int NS = tile_stages(TN);
     constexpr uint32_t kBBytes = TN * kKB;
+    static_assert((size_t)TN * kRows * 4 <= (size_t)NS * (kABytes + kBBytes), "the sums fit over the stages");
     uint8_t* A = align1024(smem_raw);
     uint8_t* B = A + (size_t)NS * kABytes;
-    int* sums = reinterpret_cast<int*>(B + (size_t)NS * kBBytes);  // [part][TN / splits][kRows]
-    uint64_t* full = reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(sums) + (splits > 1 ? TN * kRows * 4 : 0));
+    int* sums = reinterpret_cast<int*>(A);
+    uint64_t* full = reinterpret_cast<uint64_t*>(B + (size_t)NS * kBBytes);
     uint64_t* empty = full + NS;
     uint64_t* done = empty + NS;
     uint32_t* slot = reinterpret_cast<uint32_t*>(done + 1);
+    float* xs = reinterpret_cast<float*>(slot + 2);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int part = (int)(blockIdx.x % splits);
@@ -214,99 +321,112 @@ __global__ void __launch_bounds__(kThreads) int8_tile_kernel(const __grid_consta
     const int kb0 = (int)(G.kbt * part / splits), nk = (int)(G.kbt * (part + 1) / splits) - kb0;
     const Int8Product& P = G.p;
 
-    if (threadIdx.x == 0) {
-        for (int s = 0; s < NS; s++) {
-            mbar_init(&full[s], 1);
-            mbar_init(&empty[s], 1);
-        }
-        mbar_init(done, 1);
+    if (warp == 5) {
+        if (lane < 2 * NS + 1) mbar_init(full + lane, 1);  // full, empty, done
         mbar_init_fence();
+    } else if (warp == 4) {
+        if (lane < 2) prefetch_map(lane ? &G.xmap : &G.wmap);
+    } else if (warp == 0) {
+        tmem_alloc<1>(slot, TN);
     }
-    if (warp == 0) tmem_alloc<1>(slot, TN);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *slot;
-    if (splits > 1) cluster_arrive();  // the other parts may then write into this CTA's sums
     grid_dependency_wait();
     allow_dependents();
 
     bool ok = false;
     if (warp == 4) {
-        if (lane == 0) {
-            int it = 0;
-            for (; it < nk; it++) {
-                const int s = it % NS;
-                if (it >= NS && !wait_spin(&empty[s], ((it / NS) - 1) & 1, G.err)) break;
+        int it = 0;
+        for (; it < nk; it++) {
+            const int s = it % NS;
+            if (it >= NS && !wait_spin(&empty[s], ((it / NS) - 1) & 1, G.err)) break;
+            if (elect_one()) {
                 mbar_arrive_tx(&full[s], kABytes + kBBytes);
                 tensor_copy_2d(A + (size_t)s * kABytes, &G.wmap, (kb0 + it) * kKB, (int)n0, &full[s]);
                 tensor_copy_2d(B + (size_t)s * kBBytes, &G.xmap, (kb0 + it) * kKB, (int)t0, &full[s]);
             }
-            // what is in flight lands before the CTA exits
-            for (int i = it < NS ? 0 : it - NS; i < it; i++) mbar_drain(&full[i % NS], (i / NS) & 1);
+            __syncwarp();
         }
+        // what is in flight lands before the CTA exits
+        for (int i = it < NS ? 0 : it - NS; i < it; i++) mbar_drain(&full[i % NS], (i / NS) & 1);
     } else if (warp == 5) {
-        if (lane == 0) {
-            constexpr uint32_t idesc = instr_desc_i8(kRows, TN);
-            for (int it = 0; it < nk; it++) {
-                const int s = it % NS;
-                if (!wait_spin(&full[s], (it / NS) & 1, G.err)) break;
-                tc_fence_after();
-                const uint32_t a = smem_u32(A + (size_t)s * kABytes), b = smem_u32(B + (size_t)s * kBBytes);
+        constexpr uint32_t idesc = instr_desc_i8(kRows, TN);
+        for (int it = 0; it < nk; it++) {
+            const int s = it % NS;
+            if (!wait_spin(&full[s], (it / NS) & 1, G.err)) break;
+            tc_fence_after();
+            const uint32_t a = smem_u32(A + (size_t)s * kABytes), b = smem_u32(B + (size_t)s * kBBytes);
+            if (elect_one()) {
 #pragma unroll
                 for (int j = 0; j < kKB / 32; j++)
                     mma_i8<1>(tmem, smem_desc(a + 32 * j), smem_desc(b + 32 * j), idesc, it > 0 || j > 0);
                 mma_commit<1>(&empty[s]);
             }
-            mma_commit<1>(done);
-            mbar_drain(done, 0);
+            __syncwarp();
         }
+        if (elect_one()) mma_commit<1>(done);
+        __syncwarp();
+        mbar_drain(done, 0);
     } else {
+        for (int i = threadIdx.x; i < TN; i += 128) xs[i] = t0 + i < P.m ? P.xs[t0 + i] : 0.f;
+        named_sync(1, 128);
         ok = __all_sync(0xffffffffu, mbar_wait(done, 0, G.err));
         tc_fence_after();
     }
     __syncwarp();
 
-    const int64_t n = n0 + 32 * warp + lane;
     const uint32_t lanes = tmem + ((uint32_t)(32 * warp) << 16);
+    const int cols = P.m - t0 < TN ? (int)(P.m - t0) : TN;  // tokens of the tile
     if (splits == 1) {
         if (ok) {
+            const int64_t n = n0 + 32 * warp + lane;
             const float wsn = n < P.n ? P.ws[n] : 0.f;
-            for (int c = 0; c < TN && t0 + c < P.m; c += 32) {
+            for (int c = 0; c < cols; c += 32) {
                 int v[32];
                 tmem_load32(lanes + c, v);
-                emit32<OT>(P, v, n, wsn, t0 + c, lane);
+                emit32<OT>(P, v, n, wsn, t0 + c, cols - c, xs[c + lane]);
             }
         }
     } else {
-        const int own = TN / splits;  // tokens that each part finishes
-        cluster_wait();
+        const int64_t n = n0 + 4 * lane;  // four rows a lane, a token a warp
+        float wsn[4] = {};
         if (ok) {
-            const uint32_t base = smem_u32(sums) + (uint32_t)((part * own) * kRows + 32 * warp + lane) * 4;
-            for (int c = 0; c < TN && t0 + c < P.m; c += 32) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) wsn[i] = n + i < P.n ? P.ws[n + i] : 0.f;
+            for (int c = 0; c < cols; c += 32) {
                 int v[32];
                 tmem_load32(lanes + c, v);
 #pragma unroll
-                for (int j = 0; j < 32; j++) {
-                    const int col = c + j;
-                    store_cluster(map_rank(base + (uint32_t)(col % own) * kRows * 4, (uint32_t)(col / own)), v[j]);
-                }
+                for (int j = 0; j < 32; j++) sums[(c + j) * kRows + 32 * warp + lane] = v[j];
             }
         }
         cluster_arrive();
         cluster_wait();
         if (ok) {
-            const float wsn = n < P.n ? P.ws[n] : 0.f;
-            for (int c = 0; c < own; c++) {
-                const int64_t t = t0 + part * own + c;
-                if (t >= P.m || n >= P.n) break;
-                int sum = 0;
-                for (int r = 0; r < splits; r++) sum += sums[(r * own + c) * kRows + 32 * warp + lane];
-                float o = int8_scaled(sum, wsn, P.xs[t]);
-                if (P.res) o = __fadd_rn(o, P.res[t * P.ldr + n]);
-                static_cast<OT*>(P.out)[t * P.ldo + n] = int8_round<OT>(o);
+            const int c0 = TN * part / splits, c1 = min(cols, TN * (part + 1) / splits);
+            const uint32_t base = smem_u32(sums) + 16 * lane;
+            const int cnt = P.n - n < 4 ? (int)(P.n - n) : 4;
+            for (int c = c0 + warp; c < c1;) {  // eight tokens a warp at a time, then two
+                const uint32_t at = base + (uint32_t)c * kRows * 4;
+                if (c + 4 * 7 < c1) {
+                    P.res ? join_parts<OT, 8, true>(P, at, splits, t0 + c, n, cnt, wsn, xs + c)
+                          : join_parts<OT, 8, false>(P, at, splits, t0 + c, n, cnt, wsn, xs + c);
+                    c += 4 * 8;
+                } else if (c + 4 < c1) {
+                    P.res ? join_parts<OT, 2, true>(P, at, splits, t0 + c, n, cnt, wsn, xs + c)
+                          : join_parts<OT, 2, false>(P, at, splits, t0 + c, n, cnt, wsn, xs + c);
+                    c += 4 * 2;
+                } else {
+                    P.res ? join_parts<OT, 1, true>(P, at, splits, t0 + c, n, cnt, wsn, xs + c)
+                          : join_parts<OT, 1, false>(P, at, splits, t0 + c, n, cnt, wsn, xs + c);
+                    c += 4;
+                }
             }
         }
+        cluster_arrive();
+        cluster_wait();  // the other parts have read this CTA's sums
     }
     tc_fence_before();
     __syncthreads();
@@ -351,18 +471,14 @@ __global__ void __launch_bounds__(kThreads, 1) int8_pair_kernel(const __grid_con
     const int64_t tiles = G.row_tiles * G.token_tiles, first = blockIdx.x >> 1, step = gridDim.x >> 1;
     const int nk = (int)G.kbt;
 
-    if (threadIdx.x == 0) {
-        for (int s = 0; s < NS; s++) {
-            mbar_init(&full[s], 1);
-            mbar_init(&empty[s], 1);
-        }
-        for (int i = 0; i < 2; i++) {
-            mbar_init(&acc_full[i], 1);
-            mbar_init(&acc_empty[i], 8);  // the epilogue warps of both CTAs
-        }
+    if (warp == 5) {
+        if (lane < 2 * NS + 4) mbar_init(full + lane, lane < 2 * NS + 2 ? 1 : 8);  // acc_empty: both CTAs' epilogue warps
         mbar_init_fence();
+    } else if (warp == 4) {
+        if (lane < 2) prefetch_map(lane ? &G.xmap : &G.wmap);
+    } else if (warp == 0) {
+        tmem_alloc<2>(slot, 512);
     }
-    if (warp == 0) tmem_alloc<2>(slot, 512);
     tc_fence_before();
     __syncthreads();
     cluster_arrive();
@@ -373,31 +489,32 @@ __global__ void __launch_bounds__(kThreads, 1) int8_pair_kernel(const __grid_con
     allow_dependents();
 
     if (warp == 4) {
-        if (lane == 0) {
-            int64_t it = 0;
-            bool ok = true;
-            for (int64_t tile = first; tile < tiles && ok; tile += step) {
-                int64_t rt, tt;
-                pair_tile(G, tile, &rt, &tt);
-                const int y_w = (int)(rt * 2 * kRows + rank * kRows), y_x = (int)(tt * kPairTokens + rank * (kPairTokens / 2));
-                for (int kb = 0; kb < nk; kb++, it++) {
-                    const int s = (int)(it % NS);
-                    if (it >= NS && !(ok = wait_spin(&empty[s], (uint32_t)((it / NS) - 1) & 1u, G.err))) break;
+        int64_t it = 0;
+        bool ok = true;
+        for (int64_t tile = first; tile < tiles && ok; tile += step) {
+            int64_t rt, tt;
+            pair_tile(G, tile, &rt, &tt);
+            const int y_w = (int)(rt * 2 * kRows + rank * kRows), y_x = (int)(tt * kPairTokens + rank * (kPairTokens / 2));
+            for (int kb = 0; kb < nk; kb++, it++) {
+                const int s = (int)(it % NS);
+                if (it >= NS && !(ok = wait_spin(&empty[s], (uint32_t)((it / NS) - 1) & 1u, G.err))) break;
+                if (elect_one()) {
                     if (leader) mbar_arrive_tx(&full[s], 2 * (kABytes + kPairB));
                     const uint32_t bar = map_rank(smem_u32(&full[s]), 0);
                     tensor_copy_pair(A + (size_t)s * kABytes, &G.wmap, kb * kKB, y_w, bar);
                     tensor_copy_pair(B + (size_t)s * kPairB, &G.xmap, kb * kKB, y_x, bar);
                 }
+                __syncwarp();
             }
-            // every stage has been read, and the leader's commits have arrived here, before the CTA exits
-            for (int64_t i = it < NS ? 0 : it - NS; i < it && ok; i++)
-                ok = wait_spin(&empty[i % NS], (uint32_t)(i / NS) & 1u, G.err);
-            // after a wait that gave up, the copies in flight (their barrier may be the other CTA's) get
-            // 100 us to land: a thousand times what one takes
-            for (int i = 0; i < 100 && !ok; i++) __nanosleep(1000);
         }
+        // every stage has been read, and the leader's commits have arrived here, before the CTA exits
+        for (int64_t i = it < NS ? 0 : it - NS; i < it && ok; i++)
+            ok = wait_spin(&empty[i % NS], (uint32_t)(i / NS) & 1u, G.err);
+        // after a wait that gave up, the copies in flight (their barrier may be the other CTA's) get
+        // 100 us to land: a hundred times what one takes
+        for (int i = 0; i < 100 && !ok; i++) __nanosleep(1000);
     } else if (warp == 5) {
-        if (leader && lane == 0) {
+        if (leader) {
             constexpr uint32_t idesc = instr_desc_i8(2 * kRows, kPairTokens);
             int64_t it = 0, nt = 0;
             bool ok = true;
@@ -410,13 +527,17 @@ __global__ void __launch_bounds__(kThreads, 1) int8_pair_kernel(const __grid_con
                     if (!(ok = wait_spin(&full[s], (uint32_t)(it / NS) & 1u, G.err))) break;
                     tc_fence_after();
                     const uint32_t a = smem_u32(A + (size_t)s * kABytes), b = smem_u32(B + (size_t)s * kPairB);
+                    if (elect_one()) {
 #pragma unroll
-                    for (int j = 0; j < kKB / 32; j++)
-                        mma_i8<2>(tmem + (uint32_t)(buf * kPairTokens), smem_desc(a + 32 * j), smem_desc(b + 32 * j), idesc,
-                                  kb > 0 || j > 0);
-                    mma_commit<2>(&empty[s]);
+                        for (int j = 0; j < kKB / 32; j++)
+                            mma_i8<2>(tmem + (uint32_t)(buf * kPairTokens), smem_desc(a + 32 * j), smem_desc(b + 32 * j),
+                                      idesc, kb > 0 || j > 0);
+                        mma_commit<2>(&empty[s]);
+                    }
+                    __syncwarp();
                 }
-                mma_commit<2>(&acc_full[buf]);
+                if (elect_one()) mma_commit<2>(&acc_full[buf]);
+                __syncwarp();
             }
             // the MMAs issued last have read their operands before the CTA exits
             if (nt > 0) mbar_drain(&acc_full[(nt - 1) & 1], (uint32_t)((nt - 1) >> 1) & 1u);
@@ -429,13 +550,17 @@ __global__ void __launch_bounds__(kThreads, 1) int8_pair_kernel(const __grid_con
             const int buf = (int)(nt & 1);
             const int64_t n = rt * 2 * kRows + rank * kRows + 32 * warp + lane, t0 = tt * kPairTokens;
             const float wsn = n < P.n ? P.ws[n] : 0.f;
+            const int cols = P.m - t0 < kPairTokens ? (int)(P.m - t0) : kPairTokens;
+            float x = lane < cols ? P.xs[t0 + lane] : 0.f;  // the scales of the 32 tokens to come
             if (!__all_sync(0xffffffffu, mbar_wait(&acc_full[buf], (uint32_t)(nt >> 1) & 1u, G.err))) break;
             tc_fence_after();
             const uint32_t lanes = tmem + ((uint32_t)(32 * warp) << 16) + (uint32_t)(buf * kPairTokens);
-            for (int c = 0; c < kPairTokens && t0 + c < P.m; c += 32) {
+            for (int c = 0; c < cols; c += 32) {
+                const float next = c + 32 + lane < cols ? P.xs[t0 + c + 32 + lane] : 0.f;
                 int v[32];
                 tmem_load32(lanes + c, v);
-                emit32<OT>(P, v, n, wsn, t0 + c, lane);
+                emit32<OT>(P, v, n, wsn, t0 + c, cols - c, x);
+                x = next;
             }
             tc_fence_before();
             __syncwarp();
@@ -454,9 +579,18 @@ __global__ void __launch_bounds__(kThreads, 1) int8_pair_kernel(const __grid_con
 
 // ---- host -----------------------------------------------------------------------
 
+// Opts KERN into SMEM bytes of shared memory, once per device (a decoded
+// token's call takes a few microseconds, and the driver call is one of them).
 template <typename Kern>
-cudaError_t allow_smem(Kern kern, size_t smem) {
-    return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+cudaError_t allow_smem(Kern kern, size_t smem, std::atomic<uint64_t>& done) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+    if (done.load(std::memory_order_acquire) & bit) return cudaSuccess;
+    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_release);
+    return e;
 }
 
 bool make_maps(GemmI8* g, int w_box, int x_box) {
@@ -469,8 +603,9 @@ template <typename OT, int TN>
 cudaError_t launch_tile(GemmI8& g, int splits, cudaStream_t s) {
     const int64_t rt = (g.p.n + kRows - 1) / kRows, tt = (g.p.m + TN - 1) / TN;
     if (rt * splits > INT32_MAX || tt > 65535 || !make_maps(&g, kRows, TN)) return cudaErrorNotSupported;
-    const size_t smem = tile_smem(TN, splits);
-    const cudaError_t e = allow_smem(int8_tile_kernel<OT, TN>, smem);
+    const size_t smem = tile_smem(TN);
+    static std::atomic<uint64_t> allowed{0};
+    const cudaError_t e = allow_smem(int8_tile_kernel<OT, TN>, smem, allowed);
     if (e != cudaSuccess) return e;
     return launch_cluster(int8_tile_kernel<OT, TN>, dim3((unsigned)(rt * splits), (unsigned)tt), kThreads, smem, splits, s, g,
                           splits);
@@ -481,25 +616,87 @@ cudaError_t launch_pair(GemmI8& g, cudaStream_t s) {
     g.row_tiles = (g.p.n + 2 * kRows - 1) / (2 * kRows);
     g.token_tiles = (g.p.m + kPairTokens - 1) / kPairTokens;
     if (!make_maps(&g, kRows, kPairTokens / 2)) return cudaErrorNotSupported;
-    const cudaError_t e = allow_smem(int8_pair_kernel<OT>, kPairSmem);
+    static std::atomic<uint64_t> allowed{0};
+    const cudaError_t e = allow_smem(int8_pair_kernel<OT>, kPairSmem, allowed);
     if (e != cudaSuccess) return e;
     const int64_t pairs = std::min<int64_t>(g.row_tiles * g.token_tiles, sm_count() / 2);
     return launch_cluster(int8_pair_kernel<OT>, dim3((unsigned)(2 * pairs)), kThreads, kPairSmem, 2, s, g);
 }
 
+// Clusters of SPLITS tile CTAs that run at one time (an SM holds one CTA; a
+// cluster stays within a GPC, so 148 SMs hold 74 pairs but 45 threes and 33 fours).
+int resident_clusters(int splits) {
+    static std::atomic<int> known[5];
+    if (splits == 1) return sm_count();
+    if (const int n = known[splits].load()) return n;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(splits * sm_count()));
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = tile_smem(256);
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)splits;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    int n = 0;
+    static std::atomic<uint64_t> allowed{0};
+    if (allow_smem(int8_tile_kernel<float, 256>, cfg.dynamicSmemBytes, allowed) != cudaSuccess ||
+        cudaOccupancyMaxActiveClusters(&n, int8_tile_kernel<float, 256>, &cfg) != cudaSuccess || n < 1) {
+        (void)cudaGetLastError();
+        return 1;  // not known: the split looks expensive and is not taken
+    }
+    known[splits].store(n);
+    return n;
+}
+
+// The kernel for a request: the one of least time in microseconds by
+//   rounds of resident tiles x (columns of K x c + e)
+// with c a 128-byte column's time and e a tile's start and end, as measured for
+// single tiles at K = 4096 and 14336.  What it decides, at K = 4096 (us; the
+// tile is tokens / parts of K):
+//   24 tokens, 4096 rows    32/4  7.8   32/1 11.6   pair 12.6
+//   128 tokens, 4096 rows   64/2  9.8   128/1 13.4  pair 13.7
+//   256 tokens, 6144 rows   128/1 14.4  pair 15.7   256/2 16.6
+//   256 tokens, 14336 rows  pair 19.2   256/1 23.1  128/1 29.3
+//   512 tokens, 4096 rows, K = 14336:  256/2 32.1  pair 37.9  128/1 38.4
+struct Choice {
+    int tn, splits;  // tn 0: the pair kernel
+};
+Choice choose(const Int8Product& p, int64_t kbt) {
+    static const struct {
+        int tn;
+        double c, e1, es;  // es: with K split
+    } kTiles[] = {{32, 0.255, 1.4, 3.7}, {64, 0.255, 1.8, 4.4}, {128, 0.27, 2.8, 5.9}, {256, 0.34, 4.4, 8.6}};
+    const auto rounds = [](int64_t tiles, int64_t at_once) { return (double)((tiles + at_once - 1) / at_once); };
+    const int64_t pairs = ((p.n + 2 * kRows - 1) / (2 * kRows)) * ((p.m + kPairTokens - 1) / kPairTokens);
+    Choice best = {0, 1};
+    // the pair kernel's tiles overlap: only the last one's end is waited for
+    double least = rounds(pairs, sm_count() / 2) * (double)kbt * 0.275 + 4.4;
+    for (const auto& t : kTiles) {
+        const int64_t tiles = ((p.n + kRows - 1) / kRows) * ((p.m + t.tn - 1) / t.tn);
+        if ((p.m + t.tn - 1) / t.tn > 65535) continue;
+        for (int splits = 1; splits <= 4 && splits <= kbt; splits++) {
+            const double cost = rounds(tiles, resident_clusters(splits)) *
+                                ((double)((kbt + splits - 1) / splits) * t.c + (splits > 1 ? t.es : t.e1));
+            if (cost < least) {
+                least = cost;
+                best = {t.tn, splits};
+            }
+        }
+    }
+    return best;
+}
+
 template <typename OT>
 cudaError_t launch_type(GemmI8& g, cudaStream_t s) {
-    const Int8Product& p = g.p;
-    if (p.m >= 512) return launch_pair<OT>(g, s);
-    const int64_t rt = (p.n + kRows - 1) / kRows, sms = sm_count();
-    const int tn = p.m <= 32 ? 32 : p.m <= 64 ? 64 : 128;
-    const int64_t tiles = rt * ((p.m + tn - 1) / tn);
-    int splits = 1;
-    while (splits < 8 && tiles * splits * 2 <= sms && splits * 2 * 4 <= g.kbt) splits *= 2;
-    switch (tn) {
-    case 32: return launch_tile<OT, 32>(g, splits, s);
-    case 64: return launch_tile<OT, 64>(g, splits, s);
-    default: return launch_tile<OT, 128>(g, splits, s);
+    const Choice c = choose(g.p, g.kbt);
+    switch (c.tn) {
+    case 32: return launch_tile<OT, 32>(g, c.splits, s);
+    case 64: return launch_tile<OT, 64>(g, c.splits, s);
+    case 128: return launch_tile<OT, 128>(g, c.splits, s);
+    case 256: return launch_tile<OT, 256>(g, c.splits, s);
+    default: return launch_pair<OT>(g, s);
     }
 }
 

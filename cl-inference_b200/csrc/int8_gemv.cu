@@ -21,7 +21,28 @@
 namespace clq {
 namespace {
 
-constexpr int kGvWarps = 8;
+// 16 bytes of the weight stream, read once: past L1, the whole 256-byte L2
+// line asked for.  Volatile, so that the loads of a batch stay ahead of its
+// MMAs: left to the compiler's order the kernel took 8.3 us for one token at
+// 4096 x 4096, and 4.9 with this one.
+__device__ __forceinline__ uint4 load_stream(const int8_t* p) {
+    uint4 v;
+    asm volatile("ld.global.nc.L1::no_allocate.L2::256B.v4.u32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                 : "l"(p));
+    return v;
+}
+// 16 bytes of a token row, zeros where it has none.
+__device__ __forceinline__ uint4 load_token(const int8_t* p, bool in) {
+    uint4 v;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %5, 0;\n\t"
+        "mov.u32 %0, 0;\n\tmov.u32 %1, 0;\n\tmov.u32 %2, 0;\n\tmov.u32 %3, 0;\n\t"
+        "@p ld.global.v4.u32 {%0, %1, %2, %3}, [%4];\n\t}"
+        : "=&r"(v.x), "=&r"(v.y), "=&r"(v.z), "=&r"(v.w)
+        : "l"(p), "r"((uint32_t)in));
+    return v;
+}
 
 __device__ __forceinline__ void mma_s8(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                        uint32_t b1) {
@@ -39,10 +60,11 @@ __device__ __forceinline__ uint4 load_tail(const int8_t* row, int64_t k0, int64_
     return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// HI: tokens 8..15 are present.  U: 64-byte columns a warp has in flight.
-template <typename OT, int R, bool HI, int U>
-__global__ void __launch_bounds__(kGvWarps * 32) int8_gemv_kernel(const Int8Product P) {
-    __shared__ int part[kGvWarps][R][HI ? 4 : 2][32];
+// HI: tokens 8..15 are present.  R: groups of eight weight rows to a CTA.  W:
+// warps.  U: 64-byte columns a warp has in flight.
+template <typename OT, int R, bool HI, int W, int U>
+__global__ void __launch_bounds__(W * 32, 16 / W) int8_gemv_kernel(const Int8Product P) {
+    __shared__ int part[W][R][HI ? 4 : 2][32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, q = lane & 3;
     const int64_t n0 = (int64_t)blockIdx.x * 8 * R;
     pipe::grid_dependency_wait();
@@ -68,20 +90,20 @@ __global__ void __launch_bounds__(kGvWarps * 32) int8_gemv_kernel(const Int8Prod
     };
     const int64_t whole = P.k / 64;
     int64_t c = warp;
-    for (; c + (U - 1) * kGvWarps < whole; c += U * kGvWarps) {
+    for (; c + (U - 1) * W < whole; c += U * W) {
         uint4 w[U][R], a[U], b[U];
 #pragma unroll
         for (int u = 0; u < U; u++) {
-            const int64_t k0 = (c + u * kGvWarps) * 64 + 16 * q;
+            const int64_t k0 = (c + u * W) * 64 + 16 * q;
 #pragma unroll
-            for (int r = 0; r < R; r++) w[u][r] = __ldcs(reinterpret_cast<const uint4*>(wr[r] + k0));
-            a[u] = lo_in ? *reinterpret_cast<const uint4*>(xlo + k0) : zero;
-            b[u] = hi_in ? *reinterpret_cast<const uint4*>(xhi + k0) : zero;
+            for (int r = 0; r < R; r++) w[u][r] = load_stream(wr[r] + k0);
+            a[u] = load_token(xlo + k0, lo_in);
+            b[u] = HI ? load_token(xhi + k0, hi_in) : zero;
         }
 #pragma unroll
         for (int u = 0; u < U; u++) column(w[u], a[u], b[u]);
     }
-    for (; c * 64 < P.k; c += kGvWarps) {  // the last columns, one at a time
+    for (; c * 64 < P.k; c += W) {  // the last columns, one at a time
         const int64_t k0 = c * 64 + 16 * q;
         uint4 w[R];
 #pragma unroll
@@ -95,34 +117,39 @@ __global__ void __launch_bounds__(kGvWarps * 32) int8_gemv_kernel(const Int8Prod
     __syncthreads();
     // output (t, 8 r + j): lane 4 (t % 8) + j / 2, register j % 2 + 2 (t / 8)
     OT* out = static_cast<OT*>(P.out);
-    for (int e = threadIdx.x; e < (int)P.m * 8 * R; e += kGvWarps * 32) {
+    for (int e = threadIdx.x; e < (int)P.m * 8 * R; e += W * 32) {
         const int t = e / (8 * R), jn = e % (8 * R), r = jn >> 3, j = jn & 7;
         const int64_t n = n0 + jn;
         if (n >= P.n) continue;
         const int l = 4 * (t & 7) + (j >> 1), i = (j & 1) + (HI ? 2 * (t >> 3) : 0);
         int sum = 0;
 #pragma unroll
-        for (int w = 0; w < kGvWarps; w++) sum += part[w][r][i][l];
+        for (int w = 0; w < W; w++) sum += part[w][r][i][l];
         float v = int8_scaled(sum, P.ws[n], P.xs[t]);
         if (P.res) v = __fadd_rn(v, P.res[t * P.ldr + n]);
         out[t * P.ldo + n] = int8_round<OT>(v);
     }
 }
 
-template <typename OT, int R, bool HI>
+template <typename OT, int R, int W, int U>
 cudaError_t launch_gv(const Int8Product& p, cudaStream_t s) {
     const int64_t blocks = (p.n + 8 * R - 1) / (8 * R);
     if (blocks > INT32_MAX) return cudaErrorNotSupported;
-    return pipe::launch_pdl(int8_gemv_kernel<OT, R, HI, 8 / R>, dim3((unsigned)blocks), kGvWarps * 32, 0, s, p);
+    const dim3 grid((unsigned)blocks);
+    return p.m > 8 ? pipe::launch_pdl(int8_gemv_kernel<OT, R, true, W, U>, grid, W * 32, 0, s, p)
+                   : pipe::launch_pdl(int8_gemv_kernel<OT, R, false, W, U>, grid, W * 32, 0, s, p);
 }
 
+// Few rows: eight to a CTA, K over eight warps, so that every SM has a CTA (1024
+// x 4096 at one token: 2.7 us; 16 rows to a CTA 3.4).  More: 16 to a CTA, which halves
+// what the tokens' rows cost (4096 x 14336: 11.6 us, eight rows 13.6), and from
+// four CTAs an SM on four warps, whose longer runs of K keep the loads flowing
+// (14336 x 4096: 11.9 us at one token and 14.2 at sixteen, eight warps 13.2 and 15.5).
 template <typename OT>
 cudaError_t launch_gv_type(const Int8Product& p, cudaStream_t s) {
-    const bool hi = p.m > 8;
-    const int64_t sms = sm_count();
-    if (p.n >= 32 * 2 * sms) return hi ? launch_gv<OT, 4, true>(p, s) : launch_gv<OT, 4, false>(p, s);
-    if (p.n >= 16 * sms) return hi ? launch_gv<OT, 2, true>(p, s) : launch_gv<OT, 2, false>(p, s);
-    return hi ? launch_gv<OT, 1, true>(p, s) : launch_gv<OT, 1, false>(p, s);
+    const int64_t ctas16 = (p.n + 15) / 16, sms = sm_count();
+    if (ctas16 < sms) return launch_gv<OT, 1, 8, 8>(p, s);
+    return ctas16 < 4 * sms ? launch_gv<OT, 2, 8, 4>(p, s) : launch_gv<OT, 2, 4, 4>(p, s);
 }
 
 }  // namespace

@@ -23,47 +23,60 @@ _lib_swiglu = _lib.lib.clq_swiglu_quantize_device
 _lib_dequantize = _lib.lib.clq_dequantize_rows_device
 _lib_linear = _lib.lib.clq_linear_int8_device
 
-_types = None  # torch dtype -> clq_xtype
+# Filled in by _torch() at the first call: the package imports without torch.
+_t = None           # the torch module
+_types = {}         # torch dtype -> clq_xtype
+_device = None      # () -> index of the current device
+_stream = None      # device index -> handle of its current stream
 
 
 def _torch():
-    global _types
-    import torch
-    if _types is None:
-        _types = {getattr(torch, name): code for name, code in _XTYPE.items()}
-    return torch
+    global _t, _device, _stream
+    if _t is None:
+        import torch
+        _types.update((getattr(torch, name), code) for name, code in _XTYPE.items())
+        # a decoded token's call takes a few microseconds: torch's own accessors, without the objects around them
+        _device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+        _stream = getattr(torch._C, "_cuda_getCurrentRawStream", lambda d: torch.cuda.current_stream(d).cuda_stream)
+        _t = torch
+    return _t
 
 
-def _type_code(torch, dtype, what):
+def _done(status):
+    if status:
+        _lib.check(status)
+
+
+def _type_code(dtype, what):
     code = _types.get(dtype)
     if code is None:
         raise ValueError(f"{what}: float32, bfloat16 or float16, not {dtype}")
     return code
 
 
-def _matrix(torch, t, what, shape=None):
+def _matrix(t, what, shape=None):
     """T as a CUDA matrix on the current device with unit last stride."""
-    if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dim() != 2:
+    if not isinstance(t, _t.Tensor) or not t.is_cuda or t.dim() != 2:
         raise ValueError(f"{what}: a CUDA matrix")
     if shape is not None and t.shape != shape:
         raise ValueError(f"{what} is {tuple(t.shape)}, {tuple(shape)} is wanted")
-    if t.get_device() != torch.cuda.current_device():
-        raise ValueError(f"{what} lives on device {t.get_device()}, current device is {torch.cuda.current_device()}")
+    if t.get_device() != _device():
+        raise ValueError(f"{what} lives on device {t.get_device()}, current device is {_device()}")
     return t if t.stride(1) == 1 or t.shape[1] <= 1 else t.contiguous()
 
 
-def _vector(torch, t, n, what):
-    if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype != torch.float32 or t.dim() != 1 or t.shape[0] != n:
+def _vector(t, n, what):
+    if not isinstance(t, _t.Tensor) or not t.is_cuda or t.dtype != _t.float32 or t.dim() != 1 or t.shape[0] != n:
         raise ValueError(f"{what}: a CUDA float32 vector of {n}")
-    if t.get_device() != torch.cuda.current_device():
-        raise ValueError(f"{what} lives on device {t.get_device()}, current device is {torch.cuda.current_device()}")
+    if t.get_device() != _device():
+        raise ValueError(f"{what} lives on device {t.get_device()}, current device is {_device()}")
     return t if n <= 1 or t.stride(0) == 1 else t.contiguous()
 
 
-def _writable(torch, t, what, shape, dtype):
+def _writable(t, what, shape, dtype):
     """T as an output: nothing may be copied, and its rows must not share memory."""
-    if (not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype != dtype or t.shape != shape
-            or t.get_device() != torch.cuda.current_device() or (shape[1] > 1 and t.stride(1) != 1)
+    if (not isinstance(t, _t.Tensor) or not t.is_cuda or t.dtype != dtype or t.shape != shape
+            or t.get_device() != _device() or (shape[1] > 1 and t.stride(1) != 1)
             or (shape[0] > 1 and t.stride(0) < shape[1])):
         raise ValueError(f"{what}: a {dtype} matrix {tuple(shape)} on the current device, rows apart with unit last stride")
     return t
@@ -71,17 +84,18 @@ def _writable(torch, t, what, shape, dtype):
 
 def _ld(t):
     """Row stride of a matrix; a single row has none to speak of."""
-    return t.stride(0) if t.shape[0] > 1 else (t.shape[1] + 15) // 16 * 16
+    m, k = t.shape
+    return t.stride(0) if m > 1 else (k + 15) // 16 * 16
 
 
-def _on(torch, stream, tensors, call):
+def _on(stream, tensors, call):
     """CALL() with STREAM (a handle) as the current stream, so that what it
     allocates belongs to that stream; TENSORS are kept until STREAM is done."""
-    side = torch.cuda.ExternalStream(stream)
+    side = _t.cuda.ExternalStream(stream)
     for t in tensors:
         if t is not None:
             t.record_stream(side)
-    with torch.cuda.stream(side):
+    with _t.cuda.stream(side):
         return call()
 
 
@@ -91,11 +105,11 @@ class Int8Rows:
     __slots__ = ("codes", "scales")
 
     def __init__(self, codes, scales):
-        torch = _torch()
-        codes = _matrix(torch, codes, "codes")
+        torch = _t or _torch()
+        codes = _matrix(codes, "codes")
         if codes.dtype != torch.int8:
             raise ValueError(f"codes: int8, not {codes.dtype}")
-        self.codes, self.scales = codes, _vector(torch, scales, codes.shape[0], "scales")
+        self.codes, self.scales = codes, _vector(scales, codes.shape[0], "scales")
 
     @property
     def shape(self):
@@ -112,29 +126,29 @@ class Int8Rows:
 
     def dequantize(self, dtype=None, out=None, stream=None):
         """codes * scales in DTYPE (float32 without one), into OUT when given."""
-        torch = _torch()
+        torch = _t or _torch()
         if stream is not None:
-            return _on(torch, stream, (self.codes, self.scales, out), lambda: self.dequantize(dtype, out))
+            return _on(stream, (self.codes, self.scales, out), lambda: self.dequantize(dtype, out))
         m, k = self.codes.shape
         if dtype is None:
             dtype = torch.float32 if out is None else out.dtype
-        code = _type_code(torch, dtype, "dtype")
+        code = _type_code(dtype, "dtype")
         if out is None:
             out = torch.empty((m, k), dtype=dtype, device=self.codes.device)
         else:
-            _writable(torch, out, "out", (m, k), dtype)
-        _lib.check(_lib_dequantize(self.codes.data_ptr(), _ld(self.codes), self.scales.data_ptr(), m, k, out.data_ptr(),
-                                   code, _ld(out), torch.cuda.current_stream().cuda_stream))
+            _writable(out, "out", (m, k), dtype)
+        _done(_lib_dequantize(self.codes.data_ptr(), _ld(self.codes), self.scales.data_ptr(), m, k, out.data_ptr(),
+                                   code, _ld(out), _stream(_device())))
         return out
 
 
-def _empty_rows(torch, m, k, device):
+def _empty_rows(m, k, device):
     """Uninitialised Int8Rows whose code rows start on 16-byte boundaries."""
     q = Int8Rows.__new__(Int8Rows)
     pitch = (k + 15) // 16 * 16
-    codes = torch.empty((m, pitch), dtype=torch.int8, device=device)
+    codes = _t.empty((m, pitch), dtype=_t.int8, device=device)
     q.codes = codes if pitch == k else codes[:, :k]
-    q.scales = torch.empty(m, dtype=torch.float32, device=device)
+    q.scales = _t.empty(m, dtype=_t.float32, device=device)
     return q
 
 
@@ -150,52 +164,52 @@ def norm_quantize(x, norm_weight=None, eps=1e-5, residual=None, residual_out=Non
     type, or f32) x alone.  With a residual returns (rows, x + residual), the sum
     in the residual's type: RESIDUAL_OUT, which may be RESIDUAL, or a new tensor.
     """
-    torch = _torch()
+    torch = _t or _torch()
     if stream is not None:
-        return _on(torch, stream, (x, norm_weight, residual, residual_out),
+        return _on(stream, (x, norm_weight, residual, residual_out),
                    lambda: norm_quantize(x, norm_weight, eps, residual, residual_out))
-    x = _matrix(torch, x, "x")
+    x = _matrix(x, "x")
     m, k = x.shape
-    xtype = _type_code(torch, x.dtype, "x")
+    xtype = _type_code(x.dtype, "x")
     wptr = rptr = optr = None
     rtype, ldr, ldo = xtype, 0, 0
     if norm_weight is not None:
-        norm_weight = _vector(torch, norm_weight, k, "norm_weight")
+        norm_weight = _vector(norm_weight, k, "norm_weight")
         wptr = norm_weight.data_ptr()
     if residual is not None:
-        given, residual = residual, _matrix(torch, residual, "residual", x.shape)
-        rtype = _type_code(torch, residual.dtype, "residual")
+        given, residual = residual, _matrix(residual, "residual", x.shape)
+        rtype = _type_code(residual.dtype, "residual")
         if rtype not in (xtype, _lib.CLQ_X_F32):
             raise ValueError(f"residual: {x.dtype} or float32, not {residual.dtype}")
         if residual_out is None:
             residual_out = torch.empty((m, k), dtype=residual.dtype, device=x.device)
         else:
-            _writable(torch, residual_out, "residual_out", (m, k), residual.dtype)
+            _writable(residual_out, "residual_out", (m, k), residual.dtype)
             _apart(residual_out, given, "residual_out")
             _apart(residual_out, x, "residual_out")
         rptr, ldr, optr, ldo = residual.data_ptr(), _ld(residual), residual_out.data_ptr(), _ld(residual_out)
     elif residual_out is not None:
         raise ValueError("residual_out needs a residual")
-    q = _empty_rows(torch, m, k, x.device)
-    _lib.check(_lib_quantize(x.data_ptr(), xtype, m, k, _ld(x), wptr, eps, rptr, rtype, ldr, optr, ldo,
+    q = _empty_rows(m, k, x.device)
+    _done(_lib_quantize(x.data_ptr(), xtype, m, k, _ld(x), wptr, eps, rptr, rtype, ldr, optr, ldo,
                              q.codes.data_ptr(), _ld(q.codes), q.scales.data_ptr(),
-                             torch.cuda.current_stream().cuda_stream))
+                             _stream(_device())))
     return q if residual is None else (q, residual_out)
 
 
 def swiglu_quantize(gate, up, stream=None):
     """The Int8Rows of silu(gate) * up, both [m, k] of one type (two halves of one product, say)."""
-    torch = _torch()
+    torch = _t or _torch()
     if stream is not None:
-        return _on(torch, stream, (gate, up), lambda: swiglu_quantize(gate, up))
-    gate, up = _matrix(torch, gate, "gate"), _matrix(torch, up, "up", gate.shape)
+        return _on(stream, (gate, up), lambda: swiglu_quantize(gate, up))
+    gate, up = _matrix(gate, "gate"), _matrix(up, "up", gate.shape)
     if gate.dtype != up.dtype:
         raise ValueError(f"gate is {gate.dtype}, up is {up.dtype}")
-    xtype = _type_code(torch, gate.dtype, "gate")
+    xtype = _type_code(gate.dtype, "gate")
     m, k = gate.shape
-    q = _empty_rows(torch, m, k, gate.device)
-    _lib.check(_lib_swiglu(gate.data_ptr(), _ld(gate), up.data_ptr(), _ld(up), xtype, m, k, q.codes.data_ptr(),
-                           _ld(q.codes), q.scales.data_ptr(), torch.cuda.current_stream().cuda_stream))
+    q = _empty_rows(m, k, gate.device)
+    _done(_lib_swiglu(gate.data_ptr(), _ld(gate), up.data_ptr(), _ld(up), xtype, m, k, q.codes.data_ptr(),
+                           _ld(q.codes), q.scales.data_ptr(), _stream(_device())))
     return q
 
 
@@ -203,37 +217,36 @@ def linear_int8(x, w, out=None, dtype=None, residual=None, stream=None):
     """out[m, n] = X [m, k] . W [n, k]^T of two Int8Rows, plus an optional f32
     RESIDUAL [m, n] (which may be OUT), rounded once to DTYPE (OUT's, or float32).
     The products are summed in 32-bit integers: exact, for k up to 131071."""
-    torch = _torch()
+    torch = _t or _torch()
     if not isinstance(x, Int8Rows) or not isinstance(w, Int8Rows):
         raise ValueError("linear_int8 multiplies Int8Rows")
     if stream is not None:
-        return _on(torch, stream, (x.codes, x.scales, w.codes, w.scales, out, residual),
+        return _on(stream, (x.codes, x.scales, w.codes, w.scales, out, residual),
                    lambda: linear_int8(x, w, out, dtype, residual))
     m, k = x.codes.shape
     n = w.codes.shape[0]
     if w.codes.shape[1] != k:
         raise ValueError(f"rows of {k} codes against a weight of {tuple(w.codes.shape)}")
     device = x.codes.get_device()
-    if device != w.codes.get_device() or device != torch.cuda.current_device():
-        raise ValueError(f"x on device {device}, w on {w.codes.get_device()}, current device is "
-                         f"{torch.cuda.current_device()}")
+    if device != w.codes.get_device() or device != _device():
+        raise ValueError(f"x on device {device}, w on {w.codes.get_device()}, current device is {_device()}")
     if dtype is None:
         dtype = torch.float32 if out is None else out.dtype
-    code = _type_code(torch, dtype, "dtype")
+    code = _type_code(dtype, "dtype")
     if out is None:
         out = torch.empty((m, n), dtype=dtype, device=x.codes.device)
     else:
-        _writable(torch, out, "out", (m, n), dtype)
+        _writable(out, "out", (m, n), dtype)
     rptr, ldr = None, 0
     if residual is not None:
         if residual.dtype != torch.float32:
             raise ValueError(f"residual: float32, not {residual.dtype}")
-        given, residual = residual, _matrix(torch, residual, "residual", (m, n))
+        given, residual = residual, _matrix(residual, "residual", (m, n))
         _apart(out, given, "out")
         rptr, ldr = residual.data_ptr(), _ld(residual)
-    _lib.check(_lib_linear(x.codes.data_ptr(), _ld(x.codes), x.scales.data_ptr(), m, w.codes.data_ptr(), _ld(w.codes),
+    _done(_lib_linear(x.codes.data_ptr(), _ld(x.codes), x.scales.data_ptr(), m, w.codes.data_ptr(), _ld(w.codes),
                            w.scales.data_ptr(), n, k, rptr, ldr, out.data_ptr(), code, _ld(out),
-                           torch.cuda.current_stream().cuda_stream))
+                           _stream(_device())))
     return out
 
 
