@@ -40,7 +40,6 @@ constexpr int kRows = 128;                   // weight rows per CTA
 constexpr int kKB = 128;                     // codes of K per stage: one swizzle span
 constexpr uint32_t kABytes = kRows * kKB;
 constexpr int kThreads = 192;                // warps 0-3 epilogue, 4 copies, 5 MMAs
-constexpr size_t kSmemMax = 227 * 1024;
 
 struct GemmI8 {
     CUtensorMap wmap, xmap;
@@ -293,8 +292,8 @@ constexpr int tile_stages(int tn) { return tn == 256 ? 4 : tn == 128 ? 6 : tn ==
 constexpr size_t tile_smem(int tn) {
     return 1024 + (size_t)tile_stages(tn) * (kABytes + (size_t)tn * kKB) + (2 * tile_stages(tn) + 2) * 8 + (size_t)tn * 4;
 }
-static_assert(tile_smem(256) <= kSmemMax && tile_smem(128) <= kSmemMax && tile_smem(64) <= kSmemMax &&
-              tile_smem(32) <= kSmemMax, "shared memory of one SM");
+static_assert(tile_smem(256) <= kSmemPerSm && tile_smem(128) <= kSmemPerSm && tile_smem(64) <= kSmemPerSm &&
+              tile_smem(32) <= kSmemPerSm, "shared memory of one SM");
 
 // CTA (blockIdx.x = row tile x SPLITS + part, blockIdx.y = token tile); the
 // SPLITS parts of a tile form a cluster.  Each part leaves its sums in its own
@@ -441,7 +440,7 @@ __global__ void __launch_bounds__(kThreads) int8_tile_kernel(const __grid_consta
 constexpr int kPairTokens = 256, kPairStages = 6, kGroup = 8;
 constexpr uint32_t kPairB = kPairTokens / 2 * kKB;  // each CTA stages half of the tokens
 constexpr size_t kPairSmem = 1024 + (size_t)kPairStages * (kABytes + kPairB) + (2 * kPairStages + 4) * 8 + 16;
-static_assert(kPairSmem <= kSmemMax, "shared memory of one SM");
+static_assert(kPairSmem <= kSmemPerSm, "shared memory of one SM");
 
 // Tiles of 256 rows x 256 tokens in groups of kGroup row tiles, token tiles
 // outermost within a group: the tiles in flight at one time share both operands in L2.
@@ -578,20 +577,6 @@ __global__ void __launch_bounds__(kThreads, 1) int8_pair_kernel(const __grid_con
 }
 
 // ---- host -----------------------------------------------------------------------
-
-// Opts KERN into SMEM bytes of shared memory, once per device (a decoded
-// token's call takes a few microseconds, and the driver call is one of them).
-template <typename Kern>
-cudaError_t allow_smem(Kern kern, size_t smem, std::atomic<uint64_t>& done) {
-    int dev = 0;
-    cudaError_t e = cudaGetDevice(&dev);
-    if (e != cudaSuccess) return e;
-    const uint64_t bit = dev < 64 ? 1ull << dev : 0;
-    if (done.load(std::memory_order_acquire) & bit) return cudaSuccess;
-    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_release);
-    return e;
-}
 
 bool make_maps(GemmI8* g, int w_box, int x_box) {
     const Int8Product& p = g->p;

@@ -129,6 +129,53 @@ def test_strided_and_unaligned_rows(cuda, clq, xtype, offset, pitch):
     assert torch.equal(clq.quantize_rows(x[:1].expand(4, k)).codes, clq.quantize_rows(x[:1]).codes.expand(4, k))
 
 
+@pytest.mark.parametrize("m,k", [(700, 513), (3, 1500), (900, 1501), (5, 5001), (650, 5001), (2, 20001), (160, 20001),
+                                 (2, 33001)])
+@pytest.mark.parametrize("xtype,rtype", [("float32", "float32"), ("bfloat16", "bfloat16"), ("float16", "float32")])
+def test_rows_off_the_grid_at_length(cuda, clq, m, k, xtype, rtype):
+    """Rows whose starts take every distance from the 16-byte grid in turn (the row stride is odd),
+    one after another in their buffers, with the outputs' surroundings left as they were."""
+    torch = cuda
+    x = rand(torch, m * k + 8, seed=1).to(getattr(torch, xtype))[3:3 + m * k].view(m, k)
+    r = rand(torch, m * (k + 2) + 8, seed=2).to(getattr(torch, rtype))[5:5 + m * (k + 2)].view(m, k + 2)[:, :k]
+    buf = torch.full((m * (k + 4) + 8,), 7.0, dtype=r.dtype, device="cuda")
+    out = buf[1:1 + m * (k + 4)].view(m, k + 4)[:, :k]
+    g = rand(torch, k, seed=3, scale=0.3) + 1
+    h = x.double() + r.double()
+    q, total = clq.norm_quantize(x, g, 1e-5, residual=r, residual_out=out)
+    check_rows(torch, q, h * g.double(), 1 / torch.sqrt((h * h).mean(1) + 1e-5))
+    assert torch.equal(total, (x.float() + r.float()).to(r.dtype))
+    out.fill_(7.0)
+    assert (buf == 7).all()
+    check_rows(torch, clq.quantize_rows(x), x.double())
+    gate = x.flip(0).contiguous()
+    check_rows(torch, clq.swiglu_quantize(gate, x), gate.double() * torch.sigmoid(gate.double()) * x.double(), slack=1.7e-4)
+    assert status(clq) == 0
+
+
+@pytest.mark.parametrize("m", [600, 1000])
+@pytest.mark.parametrize("k", [1024, 4096, 14336])
+def test_many_rows(cuda, clq, m, k):
+    """Enough rows for the kernel that streams them, each against the same row among few."""
+    torch = cuda
+    for xtype, rtype in (("bfloat16", "float32"), ("float16", "float16"), ("float32", "float32")):
+        x = rand(torch, m, k, seed=1).to(getattr(torch, xtype))
+        r = rand(torch, m, k, seed=2).to(getattr(torch, rtype))
+        g = rand(torch, k, seed=3)
+        x[5, 7], x[m - 1, k - 1] = float("nan"), float("inf")
+        for call in (lambda a, b: clq.norm_quantize(a, g, residual=b), lambda a, b: clq.norm_quantize(a, None, residual=b),
+                     lambda a, b: (clq.quantize_rows(a), a), lambda a, b: (clq.swiglu_quantize(a, b.to(a.dtype)), a)):
+            q, t = call(x, r)
+            for at in (0, 100, m - 100):
+                few, ft = call(x[at:at + 100], r[at:at + 100])
+                assert torch.equal(q.codes[at:at + 100], few.codes)
+                far = (q.scales[at:at + 100] - few.scales).abs() / few.scales
+                assert (far.nan_to_num(0) <= (k / 64 + 20) * U).all()
+                assert torch.equal(torch.isnan(q.scales[at:at + 100]), torch.isnan(few.scales))
+                assert torch.equal(t[at:at + 100].nan_to_num(1), ft.nan_to_num(1))
+            assert torch.isnan(q.scales[[5, m - 1]]).all() and int(torch.isnan(q.scales).sum()) == 2
+
+
 @pytest.mark.parametrize("k", [40, 4096, 40000])
 @pytest.mark.parametrize("rtype", TYPES)
 def test_residual_in_place(cuda, clq, k, rtype):
@@ -185,7 +232,7 @@ def test_rows_with_nothing_or_nothing_finite(cuda, clq, k):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("m,k", [(1, 1), (3, 17), (5, 4096), (2, 5001), (70000, 3)])
+@pytest.mark.parametrize("m,k", [(1, 1), (3, 17), (5, 4096), (2, 5001), (70000, 3), (9, 700)])
 def test_dequantize(cuda, clq, dtype, m, k):
     torch = cuda
     c, s = codes_of(torch, m, k, seed=31)
