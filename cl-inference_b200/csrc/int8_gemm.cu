@@ -43,9 +43,12 @@ constexpr int kThreads = 192;                // warps 0-3 epilogue, 4 copies, 5 
 
 struct GemmI8 {
     CUtensorMap wmap, xmap;
+    CUtensorMap xmap_part;  // pair kernel: boxes of a part's tokens
     Int8Product p;
     int64_t kbt;            // 128-wide columns of K
     int64_t row_tiles, token_tiles;
+    int64_t whole;          // pair kernel: tiles taken whole; each later one in PARTS
+    int parts;
     int* err;
 };
 
@@ -442,13 +445,27 @@ constexpr uint32_t kPairB = kPairTokens / 2 * kKB;  // each CTA stages half of t
 constexpr size_t kPairSmem = 1024 + (size_t)kPairStages * (kABytes + kPairB) + (2 * kPairStages + 4) * 8 + 16;
 static_assert(kPairSmem <= kSmemPerSm, "shared memory of one SM");
 
-// Tiles of 256 rows x 256 tokens in groups of kGroup row tiles, token tiles
-// outermost within a group: the tiles in flight at one time share both operands in L2.
-__device__ __forceinline__ void pair_tile(const GemmI8& G, int64_t tile, int64_t* rt, int64_t* tt) {
+// What a pair of SMs does at one time: rows [256 RT, ..) for TOKENS tokens from T0 on.
+// The tiles of 256 rows x 256 tokens come in groups of kGroup row tiles, token
+// tiles outermost within a group, so that those in flight at one time share both
+// operands in L2.  The first G.whole of them, a multiple of the pairs, are taken
+// whole; the rest would leave pairs idle for a whole round, so each is taken in
+// G.parts ranges of its tokens.
+struct PairUnit {
+    int64_t rt, t0;
+    int tokens;
+};
+__device__ __forceinline__ PairUnit pair_unit(const GemmI8& G, int64_t unit) {
+    const int64_t late = unit - G.whole;
+    const int64_t tile = late < 0 ? unit : G.whole + late / G.parts;
     const int64_t per = kGroup * G.token_tiles, g = tile / per, i = tile - g * per;
     const int64_t left = G.row_tiles - g * kGroup, width = left < kGroup ? left : kGroup;
-    *tt = i / width;
-    *rt = g * kGroup + (i - *tt * width);
+    const int64_t tt = i / width;
+    PairUnit u;
+    u.rt = g * kGroup + (i - tt * width);
+    u.tokens = late < 0 ? kPairTokens : kPairTokens / G.parts;
+    u.t0 = tt * kPairTokens + (late < 0 ? 0 : late % G.parts * u.tokens);
+    return u;
 }
 
 template <typename OT>
@@ -467,14 +484,15 @@ __global__ void __launch_bounds__(kThreads, 1) int8_pair_kernel(const __grid_con
     const uint32_t rank = cluster_rank();
     const bool leader = rank == 0;
     const Int8Product& P = G.p;
-    const int64_t tiles = G.row_tiles * G.token_tiles, first = blockIdx.x >> 1, step = gridDim.x >> 1;
+    const int64_t tiles = G.whole + (G.row_tiles * G.token_tiles - G.whole) * G.parts;
+    const int64_t first = blockIdx.x >> 1, step = gridDim.x >> 1;
     const int nk = (int)G.kbt;
 
     if (warp == 5) {
         if (lane < 2 * NS + 4) mbar_init(full + lane, lane < 2 * NS + 2 ? 1 : 8);  // acc_empty: both CTAs' epilogue warps
         mbar_init_fence();
     } else if (warp == 4) {
-        if (lane < 2) prefetch_map(lane ? &G.xmap : &G.wmap);
+        if (lane < 3) prefetch_map(lane == 0 ? &G.wmap : lane == 1 ? &G.xmap : &G.xmap_part);
     } else if (warp == 0) {
         tmem_alloc<2>(slot, 512);
     }
@@ -491,17 +509,19 @@ __global__ void __launch_bounds__(kThreads, 1) int8_pair_kernel(const __grid_con
         int64_t it = 0;
         bool ok = true;
         for (int64_t tile = first; tile < tiles && ok; tile += step) {
-            int64_t rt, tt;
-            pair_tile(G, tile, &rt, &tt);
-            const int y_w = (int)(rt * 2 * kRows + rank * kRows), y_x = (int)(tt * kPairTokens + rank * (kPairTokens / 2));
+            const PairUnit u = pair_unit(G, tile);
+            if (u.t0 >= P.m) break;  // a part past the last token, which is a CTA's last unit
+            const int y_w = (int)(u.rt * 2 * kRows + rank * kRows), y_x = (int)(u.t0 + rank * (u.tokens / 2));
+            const CUtensorMap* xmap = u.tokens == kPairTokens ? &G.xmap : &G.xmap_part;
+            const uint32_t tx = 2u * (kABytes + (uint32_t)u.tokens / 2 * kKB);
             for (int kb = 0; kb < nk; kb++, it++) {
                 const int s = (int)(it % NS);
                 if (it >= NS && !(ok = wait_spin(&empty[s], (uint32_t)((it / NS) - 1) & 1u, G.err))) break;
                 if (elect_one()) {
-                    if (leader) mbar_arrive_tx(&full[s], 2 * (kABytes + kPairB));
+                    if (leader) mbar_arrive_tx(&full[s], tx);
                     const uint32_t bar = map_rank(smem_u32(&full[s]), 0);
                     tensor_copy_pair(A + (size_t)s * kABytes, &G.wmap, kb * kKB, y_w, bar);
-                    tensor_copy_pair(B + (size_t)s * kPairB, &G.xmap, kb * kKB, y_x, bar);
+                    tensor_copy_pair(B + (size_t)s * kPairB, xmap, kb * kKB, y_x, bar);
                 }
                 __syncwarp();
             }
@@ -514,10 +534,12 @@ __global__ void __launch_bounds__(kThreads, 1) int8_pair_kernel(const __grid_con
         for (int i = 0; i < 100 && !ok; i++) __nanosleep(1000);
     } else if (warp == 5) {
         if (leader) {
-            constexpr uint32_t idesc = instr_desc_i8(2 * kRows, kPairTokens);
             int64_t it = 0, nt = 0;
             bool ok = true;
             for (int64_t tile = first; tile < tiles && ok; tile += step, nt++) {
+                const PairUnit u = pair_unit(G, tile);
+                if (u.t0 >= P.m) break;
+                const uint32_t idesc = instr_desc_i8(2 * kRows, u.tokens);
                 const int buf = (int)(nt & 1);
                 if (nt >= 2 && !(ok = wait_spin(&acc_empty[buf], (uint32_t)((nt >> 1) - 1) & 1u, G.err))) break;
                 tc_fence_after();
@@ -544,12 +566,12 @@ __global__ void __launch_bounds__(kThreads, 1) int8_pair_kernel(const __grid_con
     } else {
         int64_t nt = 0;
         for (int64_t tile = first; tile < tiles; tile += step, nt++) {
-            int64_t rt, tt;
-            pair_tile(G, tile, &rt, &tt);
+            const PairUnit u = pair_unit(G, tile);
+            if (u.t0 >= P.m) break;
             const int buf = (int)(nt & 1);
-            const int64_t n = rt * 2 * kRows + rank * kRows + 32 * warp + lane, t0 = tt * kPairTokens;
+            const int64_t n = u.rt * 2 * kRows + rank * kRows + 32 * warp + lane, t0 = u.t0;
             const float wsn = n < P.n ? P.ws[n] : 0.f;
-            const int cols = P.m - t0 < kPairTokens ? (int)(P.m - t0) : kPairTokens;
+            const int cols = P.m - t0 < u.tokens ? (int)(P.m - t0) : u.tokens;
             float x = lane < cols ? P.xs[t0 + lane] : 0.f;  // the scales of the 32 tokens to come
             if (!__all_sync(0xffffffffu, mbar_wait(&acc_full[buf], (uint32_t)(nt >> 1) & 1u, G.err))) break;
             tc_fence_after();
@@ -596,16 +618,28 @@ cudaError_t launch_tile(GemmI8& g, int splits, cudaStream_t s) {
                           splits);
 }
 
+// Into how many parts (1, 2, 4 or 8) each of LATE tiles goes so that PAIRS take them in one round.
+int parts_of(int64_t late, int64_t pairs) {
+    int parts = 1;
+    while (parts < 8 && late * parts * 2 <= pairs) parts *= 2;
+    return parts;
+}
+
 template <typename OT>
 cudaError_t launch_pair(GemmI8& g, cudaStream_t s) {
     g.row_tiles = (g.p.n + 2 * kRows - 1) / (2 * kRows);
     g.token_tiles = (g.p.m + kPairTokens - 1) / kPairTokens;
-    if (!make_maps(&g, kRows, kPairTokens / 2)) return cudaErrorNotSupported;
+    const int64_t tiles = g.row_tiles * g.token_tiles, pairs = sm_count() / 2;
+    g.whole = tiles / pairs * pairs;
+    g.parts = parts_of(tiles - g.whole, pairs);
+    if (!make_maps(&g, kRows, kPairTokens / 2) ||
+        !encode_swizzled_rows(&g.xmap_part, g.p.x, g.p.m, g.p.k, g.p.ldx, kPairTokens / 2 / g.parts))
+        return cudaErrorNotSupported;
     static std::atomic<uint64_t> allowed{0};
     const cudaError_t e = allow_smem(int8_pair_kernel<OT>, kPairSmem, allowed);
     if (e != cudaSuccess) return e;
-    const int64_t pairs = std::min<int64_t>(g.row_tiles * g.token_tiles, sm_count() / 2);
-    return launch_cluster(int8_pair_kernel<OT>, dim3((unsigned)(2 * pairs)), kThreads, kPairSmem, 2, s, g);
+    const int64_t units = g.whole + (tiles - g.whole) * g.parts;
+    return launch_cluster(int8_pair_kernel<OT>, dim3((unsigned)(2 * std::min(units, pairs))), kThreads, kPairSmem, 2, s, g);
 }
 
 // Clusters of SPLITS tile CTAs that run at one time (an SM holds one CTA; a
@@ -654,10 +688,13 @@ Choice choose(const Int8Product& p, int64_t kbt) {
         double c, e1, es;  // es: with K split
     } kTiles[] = {{32, 0.255, 1.4, 3.7}, {64, 0.255, 1.8, 4.4}, {128, 0.27, 2.8, 5.9}, {256, 0.34, 4.4, 8.6}};
     const auto rounds = [](int64_t tiles, int64_t at_once) { return (double)((tiles + at_once - 1) / at_once); };
-    const int64_t pairs = ((p.n + 2 * kRows - 1) / (2 * kRows)) * ((p.m + kPairTokens - 1) / kPairTokens);
+    const int64_t units = ((p.n + 2 * kRows - 1) / (2 * kRows)) * ((p.m + kPairTokens - 1) / kPairTokens);
+    const int64_t pairs = sm_count() / 2;
+    const int parts = parts_of(units % pairs, pairs);
     Choice best = {0, 1};
     // the pair kernel's tiles overlap: only the last one's end is waited for
-    double least = rounds(pairs, sm_count() / 2) * (double)kbt * 0.275 + 4.4;
+    double least = (double)kbt * (0.275 * (double)(units / pairs) + (units % pairs ? 0.14 + 0.135 / parts : 0.)) +
+                   (units % pairs ? 1.4 + 3.0 / parts : 4.4);
     for (const auto& t : kTiles) {
         const int64_t tiles = ((p.n + kRows - 1) / kRows) * ((p.m + t.tn - 1) / t.tn);
         if ((p.m + t.tn - 1) / t.tn > 65535) continue;

@@ -60,16 +60,14 @@ def _matrix(t, what, shape=None):
         raise ValueError(f"{what}: a CUDA matrix")
     if shape is not None and t.shape != shape:
         raise ValueError(f"{what} is {tuple(t.shape)}, {tuple(shape)} is wanted")
-    if t.get_device() != _device():
-        raise ValueError(f"{what} lives on device {t.get_device()}, current device is {_device()}")
+    _here(t, what)
     return t if t.stride(1) == 1 or t.shape[1] <= 1 else t.contiguous()
 
 
 def _vector(t, n, what):
     if not isinstance(t, _t.Tensor) or not t.is_cuda or t.dtype != _t.float32 or t.dim() != 1 or t.shape[0] != n:
         raise ValueError(f"{what}: a CUDA float32 vector of {n}")
-    if t.get_device() != _device():
-        raise ValueError(f"{what} lives on device {t.get_device()}, current device is {_device()}")
+    _here(t, what)
     return t if n <= 1 or t.stride(0) == 1 else t.contiguous()
 
 
@@ -82,9 +80,16 @@ def _writable(t, what, shape, dtype):
     return t
 
 
-def _ld(t):
-    """Row stride of a matrix; a single row has none to speak of."""
-    m, k = t.shape
+def _here(t, what):
+    """The current device's index, which must be T's."""
+    device = _device()
+    if t.get_device() != device:
+        raise ValueError(f"{what} lives on device {t.get_device()}, current device is {device}")
+    return device
+
+
+def _ld(t, m, k):
+    """Row stride of an [M, K] matrix; a single row has none to speak of."""
     return t.stride(0) if m > 1 else (k + 15) // 16 * 16
 
 
@@ -127,29 +132,32 @@ class Int8Rows:
     def dequantize(self, dtype=None, out=None, stream=None):
         """codes * scales in DTYPE (float32 without one), into OUT when given."""
         torch = _t or _torch()
+        codes, scales = self.codes, self.scales
         if stream is not None:
-            return _on(stream, (self.codes, self.scales, out), lambda: self.dequantize(dtype, out))
-        m, k = self.codes.shape
+            return _on(stream, (codes, scales, out), lambda: self.dequantize(dtype, out))
+        m, k = codes.shape
+        device = _here(codes, "codes")
         if dtype is None:
             dtype = torch.float32 if out is None else out.dtype
         code = _type_code(dtype, "dtype")
         if out is None:
-            out = torch.empty((m, k), dtype=dtype, device=self.codes.device)
+            out = codes.new_empty((m, k), dtype=dtype)
         else:
             _writable(out, "out", (m, k), dtype)
-        _done(_lib_dequantize(self.codes.data_ptr(), _ld(self.codes), self.scales.data_ptr(), m, k, out.data_ptr(),
-                                   code, _ld(out), _stream(_device())))
+        _done(_lib_dequantize(codes.data_ptr(), _ld(codes, m, k), scales.data_ptr(), m, k, out.data_ptr(), code,
+                              _ld(out, m, k), _stream(device)))
         return out
 
 
-def _empty_rows(m, k, device):
-    """Uninitialised Int8Rows whose code rows start on 16-byte boundaries."""
+def _empty_rows(x, m, k):
+    """Uninitialised Int8Rows beside X whose code rows start on 16-byte
+    boundaries, and their row stride."""
     q = Int8Rows.__new__(Int8Rows)
     pitch = (k + 15) // 16 * 16
-    codes = _t.empty((m, pitch), dtype=_t.int8, device=device)
+    codes = x.new_empty((m, pitch), dtype=_t.int8)
     q.codes = codes if pitch == k else codes[:, :k]
-    q.scales = _t.empty(m, dtype=_t.float32, device=device)
-    return q
+    q.scales = x.new_empty(m, dtype=_t.float32)
+    return q, pitch
 
 
 def quantize_rows(x, stream=None):
@@ -182,24 +190,24 @@ def norm_quantize(x, norm_weight=None, eps=1e-5, residual=None, residual_out=Non
         if rtype not in (xtype, _lib.CLQ_X_F32):
             raise ValueError(f"residual: {x.dtype} or float32, not {residual.dtype}")
         if residual_out is None:
-            residual_out = torch.empty((m, k), dtype=residual.dtype, device=x.device)
+            residual_out = torch.empty_like(residual, memory_format=torch.contiguous_format)
         else:
             _writable(residual_out, "residual_out", (m, k), residual.dtype)
             _apart(residual_out, given, "residual_out")
             _apart(residual_out, x, "residual_out")
-        rptr, ldr, optr, ldo = residual.data_ptr(), _ld(residual), residual_out.data_ptr(), _ld(residual_out)
+        rptr, ldr = residual.data_ptr(), _ld(residual, m, k)
+        optr, ldo = residual_out.data_ptr(), _ld(residual_out, m, k)
     elif residual_out is not None:
         raise ValueError("residual_out needs a residual")
-    q = _empty_rows(m, k, x.device)
-    _done(_lib_quantize(x.data_ptr(), xtype, m, k, _ld(x), wptr, eps, rptr, rtype, ldr, optr, ldo,
-                             q.codes.data_ptr(), _ld(q.codes), q.scales.data_ptr(),
-                             _stream(_device())))
+    q, pitch = _empty_rows(x, m, k)
+    _done(_lib_quantize(x.data_ptr(), xtype, m, k, _ld(x, m, k), wptr, eps, rptr, rtype, ldr, optr, ldo, q.codes.data_ptr(),
+                        pitch, q.scales.data_ptr(), _stream(_device())))
     return q if residual is None else (q, residual_out)
 
 
 def swiglu_quantize(gate, up, stream=None):
     """The Int8Rows of silu(gate) * up, both [m, k] of one type (two halves of one product, say)."""
-    torch = _t or _torch()
+    _t or _torch()
     if stream is not None:
         return _on(stream, (gate, up), lambda: swiglu_quantize(gate, up))
     gate, up = _matrix(gate, "gate"), _matrix(up, "up", gate.shape)
@@ -207,9 +215,9 @@ def swiglu_quantize(gate, up, stream=None):
         raise ValueError(f"gate is {gate.dtype}, up is {up.dtype}")
     xtype = _type_code(gate.dtype, "gate")
     m, k = gate.shape
-    q = _empty_rows(m, k, gate.device)
-    _done(_lib_swiglu(gate.data_ptr(), _ld(gate), up.data_ptr(), _ld(up), xtype, m, k, q.codes.data_ptr(),
-                           _ld(q.codes), q.scales.data_ptr(), _stream(_device())))
+    q, pitch = _empty_rows(gate, m, k)
+    _done(_lib_swiglu(gate.data_ptr(), _ld(gate, m, k), up.data_ptr(), _ld(up, m, k), xtype, m, k, q.codes.data_ptr(), pitch,
+                      q.scales.data_ptr(), _stream(_device())))
     return q
 
 
@@ -223,30 +231,30 @@ def linear_int8(x, w, out=None, dtype=None, residual=None, stream=None):
     if stream is not None:
         return _on(stream, (x.codes, x.scales, w.codes, w.scales, out, residual),
                    lambda: linear_int8(x, w, out, dtype, residual))
-    m, k = x.codes.shape
-    n = w.codes.shape[0]
-    if w.codes.shape[1] != k:
-        raise ValueError(f"rows of {k} codes against a weight of {tuple(w.codes.shape)}")
-    device = x.codes.get_device()
-    if device != w.codes.get_device() or device != _device():
-        raise ValueError(f"x on device {device}, w on {w.codes.get_device()}, current device is {_device()}")
+    xc, wc = x.codes, w.codes
+    m, k = xc.shape
+    n, wk = wc.shape
+    if wk != k:
+        raise ValueError(f"rows of {k} codes against a weight of {tuple(wc.shape)}")
+    device = _here(xc, "x")
+    _here(wc, "w")
     if dtype is None:
         dtype = torch.float32 if out is None else out.dtype
     code = _type_code(dtype, "dtype")
-    if out is None:
-        out = torch.empty((m, n), dtype=dtype, device=x.codes.device)
-    else:
-        _writable(out, "out", (m, n), dtype)
     rptr, ldr = None, 0
+    if out is not None:
+        _writable(out, "out", (m, n), dtype)
     if residual is not None:
+        if out is not None:
+            _apart(out, residual, "out")
+        residual = _matrix(residual, "residual", (m, n))
         if residual.dtype != torch.float32:
             raise ValueError(f"residual: float32, not {residual.dtype}")
-        given, residual = residual, _matrix(residual, "residual", (m, n))
-        _apart(out, given, "out")
-        rptr, ldr = residual.data_ptr(), _ld(residual)
-    _done(_lib_linear(x.codes.data_ptr(), _ld(x.codes), x.scales.data_ptr(), m, w.codes.data_ptr(), _ld(w.codes),
-                           w.scales.data_ptr(), n, k, rptr, ldr, out.data_ptr(), code, _ld(out),
-                           _stream(_device())))
+        rptr, ldr = residual.data_ptr(), _ld(residual, m, n)
+    if out is None:
+        out = xc.new_empty((m, n), dtype=dtype)
+    _done(_lib_linear(xc.data_ptr(), _ld(xc, m, k), x.scales.data_ptr(), m, wc.data_ptr(), _ld(wc, n, k), w.scales.data_ptr(), n,
+                      k, rptr, ldr, out.data_ptr(), code, _ld(out, m, n), _stream(device)))
     return out
 
 
