@@ -291,7 +291,9 @@ __device__ __forceinline__ void join_parts(const Int8Product& P, uint32_t at, in
 
 // ---- tile kernel --------------------------------------------------------------
 
-constexpr int tile_stages(int tn) { return tn == 256 ? 4 : tn == 128 ? 6 : tn == 64 ? 8 : 10; }
+// 32 tokens: half of an SM's shared memory, so that the next launch's CTAs can
+// start beside the last ones (24 x 4096 x 4096: 7.4 us, with ten stages 7.7).
+constexpr int tile_stages(int tn) { return tn == 256 ? 4 : tn == 128 ? 6 : tn == 64 ? 8 : 5; }
 constexpr size_t tile_smem(int tn) {
     return 1024 + (size_t)tile_stages(tn) * (kABytes + (size_t)tn * kKB) + (2 * tile_stages(tn) + 2) * 8 + (size_t)tn * 4;
 }
@@ -642,10 +644,11 @@ cudaError_t launch_pair(GemmI8& g, cudaStream_t s) {
     return launch_cluster(int8_pair_kernel<OT>, dim3((unsigned)(2 * std::min(units, pairs))), kThreads, kPairSmem, 2, s, g);
 }
 
-// Clusters of SPLITS tile CTAs that run at one time (an SM holds one CTA; a
-// cluster stays within a GPC, so 148 SMs hold 74 pairs but 45 threes and 33 fours).
+// Clusters of SPLITS tile CTAs that run at one time, counting one CTA to an SM (a
+// cluster stays within a GPC: 148 SMs hold 74 pairs but 45 threes and 33 fours).
+constexpr int kMaxSplits = 8;
 int resident_clusters(int splits) {
-    static std::atomic<int> known[5];
+    static std::atomic<int> known[kMaxSplits + 1];
     if (splits == 1) return sm_count();
     if (const int n = known[splits].load()) return n;
     cudaLaunchConfig_t cfg = {};
@@ -670,15 +673,15 @@ int resident_clusters(int splits) {
 }
 
 // The kernel for a request: the one of least time in microseconds by
-//   rounds of resident tiles x (columns of K x c + e)
-// with c a 128-byte column's time and e a tile's start and end, as measured for
-// single tiles at K = 4096 and 14336.  What it decides, at K = 4096 (us; the
-// tile is tokens / parts of K):
-//   24 tokens, 4096 rows    32/4  7.8   32/1 11.6   pair 12.6
-//   128 tokens, 4096 rows   64/2  9.8   128/1 13.4  pair 13.7
-//   256 tokens, 6144 rows   128/1 14.4  pair 15.7   256/2 16.6
-//   256 tokens, 14336 rows  pair 19.2   256/1 23.1  128/1 29.3
-//   512 tokens, 4096 rows, K = 14336:  256/2 32.1  pair 37.9  128/1 38.4
+//   max(rounds of resident tiles x columns of K x c, traffic) + rounds x e
+// with c a 128-byte column's time and e a tile's start and end, fitted to every
+// variant at 1024 to 14336 rows and K = 2051 to 14336.  What it decides, at K =
+// 4096 (us; the tile kernel as tokens / parts of K):
+//   24 tokens, 4096 rows    32/4  7.4   32/1 11.6   pair 12.9
+//   128 tokens, 4096 rows   64/2  9.8   128/1 13.4  pair 13.6
+//   256 tokens, 6144 rows   128/1 14.2  pair 15.1   256/2 16.4
+//   256 tokens, 14336 rows  pair 19.4   256/1 22.2  128/1 28.5
+//   512 tokens, 4096 rows, K = 14336:  256/2 31.9  128/1 37.1  pair 37.7
 struct Choice {
     int tn, splits;  // tn 0: the pair kernel
 };
@@ -686,21 +689,24 @@ Choice choose(const Int8Product& p, int64_t kbt) {
     static const struct {
         int tn;
         double c, e1, es;  // es: with K split
-    } kTiles[] = {{32, 0.255, 1.4, 3.7}, {64, 0.255, 1.8, 4.4}, {128, 0.27, 2.8, 5.9}, {256, 0.34, 4.4, 8.6}};
+    } kTiles[] = {{32, 0.255, 1.2, 2.6}, {64, 0.255, 1.8, 3.4}, {128, 0.27, 2.8, 5.0}, {256, 0.34, 4.4, 8.4}};
+    static const int kSplits[] = {1, 2, 3, 4, 6, 8};
     const auto rounds = [](int64_t tiles, int64_t at_once) { return (double)((tiles + at_once - 1) / at_once); };
+    const double traffic = (double)(p.n + p.m) * (double)p.k / 6.2e6;
     const int64_t units = ((p.n + 2 * kRows - 1) / (2 * kRows)) * ((p.m + kPairTokens - 1) / kPairTokens);
     const int64_t pairs = sm_count() / 2;
     const int parts = parts_of(units % pairs, pairs);
+    // the pair kernel's tiles overlap: only the last one's end, shorter in parts, is waited for
     Choice best = {0, 1};
-    // the pair kernel's tiles overlap: only the last one's end is waited for
-    double least = (double)kbt * (0.275 * (double)(units / pairs) + (units % pairs ? 0.14 + 0.135 / parts : 0.)) +
-                   (units % pairs ? 1.4 + 3.0 / parts : 4.4);
+    double least = (double)kbt * (0.35 * (double)(units / pairs) + (units % pairs ? parts > 1 ? 0.28 : 0.335 : 0.));
+    least = std::max(least, traffic) + (units % pairs == 0 || parts == 1 ? 4.5 : parts == 2 ? 4.0 : parts == 4 ? 2.8 : 2.5);
     for (const auto& t : kTiles) {
         const int64_t tiles = ((p.n + kRows - 1) / kRows) * ((p.m + t.tn - 1) / t.tn);
         if ((p.m + t.tn - 1) / t.tn > 65535) continue;
-        for (int splits = 1; splits <= 4 && splits <= kbt; splits++) {
-            const double cost = rounds(tiles, resident_clusters(splits)) *
-                                ((double)((kbt + splits - 1) / splits) * t.c + (splits > 1 ? t.es : t.e1));
+        for (const int splits : kSplits) {
+            if (splits > 1 && 2 * splits > kbt) break;
+            const double r = rounds(tiles, resident_clusters(splits));
+            const double cost = std::max(r * (double)((kbt + splits - 1) / splits) * t.c, traffic) + r * (splits > 1 ? t.es : t.e1);
             if (cost < least) {
                 least = cost;
                 best = {t.tn, splits};

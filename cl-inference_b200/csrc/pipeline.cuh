@@ -106,6 +106,10 @@ __device__ __forceinline__ void tensor_copy_3d_hint(void* dst, const void* map, 
         "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar)), "l"(policy)
         : "memory");
 }
+// BYTES (a multiple of 16) at SRC (16-byte aligned, global) brought into L2.
+__device__ __forceinline__ void prefetch_l2(const void* src, uint32_t bytes) {
+    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(src), "r"(bytes) : "memory");
+}
 // Programmatic dependent launch: wait until the grids this one depends on
 // have completed and their writes are visible (a no-op without the launch
 // attribute), and let the next grid in the stream start its prologue.

@@ -42,16 +42,18 @@ def _torch():
     return _t
 
 
-def _done(status):
-    if status:
-        _lib.check(status)
-
-
 def _type_code(dtype, what):
     code = _types.get(dtype)
     if code is None:
         raise ValueError(f"{what}: float32, bfloat16 or float16, not {dtype}")
     return code
+
+
+def _plain(t, dtype, dims):
+    """Whether T is a tensor of that type and rank on the current device with
+    unit last stride: what nearly every call has, told in one go."""
+    return (type(t) is _t.Tensor and t.dtype is dtype and t.dim() == dims and t.is_cuda and t.get_device() == _device()
+            and t.stride(-1) == 1)
 
 
 def _matrix(t, what, shape=None):
@@ -111,10 +113,13 @@ class Int8Rows:
 
     def __init__(self, codes, scales):
         torch = _t or _torch()
-        codes = _matrix(codes, "codes")
-        if codes.dtype != torch.int8:
-            raise ValueError(f"codes: int8, not {codes.dtype}")
-        self.codes, self.scales = codes, _vector(scales, codes.shape[0], "scales")
+        if not _plain(codes, torch.int8, 2):
+            codes = _matrix(codes, "codes")
+            if codes.dtype != torch.int8:
+                raise ValueError(f"codes: int8, not {codes.dtype}")
+        if not _plain(scales, torch.float32, 1) or scales.shape[0] != codes.shape[0]:
+            scales = _vector(scales, codes.shape[0], "scales")
+        self.codes, self.scales = codes, scales
 
     @property
     def shape(self):
@@ -144,8 +149,10 @@ class Int8Rows:
             out = codes.new_empty((m, k), dtype=dtype)
         else:
             _writable(out, "out", (m, k), dtype)
-        _done(_lib_dequantize(codes.data_ptr(), _ld(codes, m, k), scales.data_ptr(), m, k, out.data_ptr(), code,
-                              _ld(out, m, k), _stream(device)))
+        status = _lib_dequantize(codes.data_ptr(), _ld(codes, m, k), scales.data_ptr(), m, k, out.data_ptr(), code,
+                                 _ld(out, m, k), _stream(device))
+        if status:
+            _lib.check(status)
         return out
 
 
@@ -176,16 +183,22 @@ def norm_quantize(x, norm_weight=None, eps=1e-5, residual=None, residual_out=Non
     if stream is not None:
         return _on(stream, (x, norm_weight, residual, residual_out),
                    lambda: norm_quantize(x, norm_weight, eps, residual, residual_out))
-    x = _matrix(x, "x")
+    if not _plain(x, getattr(x, "dtype", None), 2):
+        x = _matrix(x, "x")
     m, k = x.shape
-    xtype = _type_code(x.dtype, "x")
+    xtype = _types.get(x.dtype)
+    if xtype is None:
+        _type_code(x.dtype, "x")
     wptr = rptr = optr = None
     rtype, ldr, ldo = xtype, 0, 0
     if norm_weight is not None:
-        norm_weight = _vector(norm_weight, k, "norm_weight")
+        if not _plain(norm_weight, torch.float32, 1) or norm_weight.shape[0] != k:
+            norm_weight = _vector(norm_weight, k, "norm_weight")
         wptr = norm_weight.data_ptr()
     if residual is not None:
-        given, residual = residual, _matrix(residual, "residual", x.shape)
+        given = residual
+        if not _plain(residual, getattr(residual, "dtype", None), 2) or residual.shape != x.shape:
+            residual = _matrix(residual, "residual", x.shape)
         rtype = _type_code(residual.dtype, "residual")
         if rtype not in (xtype, _lib.CLQ_X_F32):
             raise ValueError(f"residual: {x.dtype} or float32, not {residual.dtype}")
@@ -200,8 +213,10 @@ def norm_quantize(x, norm_weight=None, eps=1e-5, residual=None, residual_out=Non
     elif residual_out is not None:
         raise ValueError("residual_out needs a residual")
     q, pitch = _empty_rows(x, m, k)
-    _done(_lib_quantize(x.data_ptr(), xtype, m, k, _ld(x, m, k), wptr, eps, rptr, rtype, ldr, optr, ldo, q.codes.data_ptr(),
-                        pitch, q.scales.data_ptr(), _stream(_device())))
+    status = _lib_quantize(x.data_ptr(), xtype, m, k, _ld(x, m, k), wptr, eps, rptr, rtype, ldr, optr, ldo, q.codes.data_ptr(),
+                           pitch, q.scales.data_ptr(), _stream(_device()))
+    if status:
+        _lib.check(status)
     return q if residual is None else (q, residual_out)
 
 
@@ -210,14 +225,19 @@ def swiglu_quantize(gate, up, stream=None):
     _t or _torch()
     if stream is not None:
         return _on(stream, (gate, up), lambda: swiglu_quantize(gate, up))
-    gate, up = _matrix(gate, "gate"), _matrix(up, "up", gate.shape)
+    if not _plain(gate, getattr(gate, "dtype", None), 2):
+        gate = _matrix(gate, "gate")
+    if not _plain(up, getattr(up, "dtype", None), 2) or up.shape != gate.shape:
+        up = _matrix(up, "up", gate.shape)
     if gate.dtype != up.dtype:
         raise ValueError(f"gate is {gate.dtype}, up is {up.dtype}")
     xtype = _type_code(gate.dtype, "gate")
     m, k = gate.shape
     q, pitch = _empty_rows(gate, m, k)
-    _done(_lib_swiglu(gate.data_ptr(), _ld(gate, m, k), up.data_ptr(), _ld(up, m, k), xtype, m, k, q.codes.data_ptr(), pitch,
-                      q.scales.data_ptr(), _stream(_device())))
+    status = _lib_swiglu(gate.data_ptr(), _ld(gate, m, k), up.data_ptr(), _ld(up, m, k), xtype, m, k, q.codes.data_ptr(), pitch,
+                         q.scales.data_ptr(), _stream(_device()))
+    if status:
+        _lib.check(status)
     return q
 
 
@@ -237,7 +257,8 @@ def linear_int8(x, w, out=None, dtype=None, residual=None, stream=None):
     if wk != k:
         raise ValueError(f"rows of {k} codes against a weight of {tuple(wc.shape)}")
     device = _here(xc, "x")
-    _here(wc, "w")
+    if wc.get_device() != device:
+        _here(wc, "w")
     if dtype is None:
         dtype = torch.float32 if out is None else out.dtype
     code = _type_code(dtype, "dtype")
@@ -253,8 +274,10 @@ def linear_int8(x, w, out=None, dtype=None, residual=None, stream=None):
         rptr, ldr = residual.data_ptr(), _ld(residual, m, n)
     if out is None:
         out = xc.new_empty((m, n), dtype=dtype)
-    _done(_lib_linear(xc.data_ptr(), _ld(xc, m, k), x.scales.data_ptr(), m, wc.data_ptr(), _ld(wc, n, k), w.scales.data_ptr(), n,
-                      k, rptr, ldr, out.data_ptr(), code, _ld(out, m, n), _stream(device)))
+    status = _lib_linear(xc.data_ptr(), _ld(xc, m, k), x.scales.data_ptr(), m, wc.data_ptr(), _ld(wc, n, k), w.scales.data_ptr(),
+                         n, k, rptr, ldr, out.data_ptr(), code, _ld(out, m, n), _stream(device))
+    if status:
+        _lib.check(status)
     return out
 
 
