@@ -41,22 +41,22 @@ __device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
 
 // silu(g) * u = g / (1 + 2^(-g log2 e)) * u.  The exponent's product is kept in
 // two parts (t and what its rounding left), so that the relative error stays that
-// of ex2.approx (2^-22) for every gate, and the reciprocal gets one Newton step: 8
-// roundings of 2^-24 in all, where the library's exponential and an IEEE
-// quotient have 7 and take three times the instructions (2048 rows of 14336: 235 us
-// with those, 34 with these).  From 2^126 on the quotient is below |g| 2^-126 and
-// counts as 0.  A gate that is not finite stays so: v becomes NaN or infinite.
+// of ex2.approx (2^-22) for every gate; with rcp.approx (2^-23) and four f32
+// roundings v is within 10 roundings of 2^-24, where the library's exponential and
+// an IEEE quotient have 7 and cost three times the instructions, which bound this
+// kernel (2048 rows of 14336 bf16: 235 us in the first form, 35 now).  Gates
+// below -87 count as -87 in the quotient, whose value there is under 2^-125.  A
+// gate that is not finite stays so: v becomes NaN or infinite.
 __device__ __forceinline__ float silu_times(float g, float u) {
     constexpr float kLog2e = 1.44269504f, kLog2eLow = 1.92596303e-8f, kLn2 = 0.693147181f;
-    const float t = __fmul_rn(-g, kLog2e);
-    const float low = fmaf(-g, kLog2eLow, fmaf(-g, kLog2e, -t));
-    float e;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(fminf(t, 126.f)));
+    const float n = -fminf(fmaxf(g, -87.f), 200.f);
+    const float t = __fmul_rn(n, kLog2e);
+    const float low = fmaf(n, kLog2eLow, fmaf(n, kLog2e, -t));
+    float e, r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
     const float d = 1.f + fmaf(e, low * kLn2, e);
-    float r;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d));
-    r = fmaf(r, fmaf(-d, r, 1.f), r);
-    return __fmul_rn(__fmul_rn(g, t > 126.f ? 0.f : r), u);
+    return __fmul_rn(__fmul_rn(g, r), u);
 }
 
 // max(a, |v|), NaN once either is.
@@ -155,20 +155,23 @@ __device__ __forceinline__ float2 row_reduce_cta(float ss, float peak, float2* r
     return row_reduce_warp(a.x, a.y);
 }
 
-// The codes of V values at P (on 4 or 8 bytes for V = 4 or 8).
+// The codes of V values at P (on 4 or 8 bytes for V = 4 or 8); zeros for inv 0,
+// whose values may be anything.
 template <int V>
 __device__ __forceinline__ void store_codes(int8_t* p, const float (&v)[V], float inv) {
-    uint32_t b[V];
-#pragma unroll
-    for (int j = 0; j < V; j++) b[j] = inv > 0.f ? code_bits(v[j], inv) : 0u;
     if constexpr (V == 1) {
-        *p = (int8_t)b[0];
+        *p = inv > 0.f ? (int8_t)code_bits(v[0], inv) : (int8_t)0;
     } else {
-        uint32_t w[V / 4];
+        uint32_t w[V / 4] = {};
+        if (inv > 0.f) {  // the same for the whole row
 #pragma unroll
-        for (int q = 0; q < V / 4; q++)
-            w[q] = __byte_perm(__byte_perm(b[4 * q], b[4 * q + 1], 0x0040), __byte_perm(b[4 * q + 2], b[4 * q + 3], 0x0040),
-                               0x5410);
+            for (int q = 0; q < V / 4; q++) {
+                uint32_t b[4];
+#pragma unroll
+                for (int j = 0; j < 4; j++) b[j] = code_bits(v[4 * q + j], inv);
+                w[q] = __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
+            }
+        }
         if constexpr (V == 4) *reinterpret_cast<uint32_t*>(p) = w[0];
         else *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
     }
@@ -266,8 +269,12 @@ __global__ void __launch_bounds__(G == 32 ? kSmallRow : G, min_ctas<XT, step_of<
 // ---- many rows, streamed through shared memory ------------------------------
 
 constexpr int kStreamStages = 4;
-constexpr int kStreamHeader = 512;  // barriers and two rows' reductions
-constexpr int kStreamThreads = 512;
+constexpr int kStreamHeader = 1024;  // barriers and two rows' reductions
+// Threads of a CTA at most: rows off the grid, whose reads are longer, gain by more
+// of them (SwiGLU of 700 x 20001 bf16 26.4 us, with 512 30.4), the others lose (2048 x
+// 14336 37.0, with 1024 39.8).
+constexpr int stream_threads(bool loose) { return loose ? 1024 : 512; }
+constexpr int stream_values(bool loose) { return loose ? 32 : 64; }  // of a thread at most
 
 // W[0, N) = the N words that start BYTES (under 16) into W[0, N + 4).
 template <int N, bool ODD_HALVES>
@@ -376,12 +383,14 @@ __device__ __forceinline__ void store_shifted(T* p, int i, int k, const float (&
 // CTA b takes rows b, b + gridDim.x, ..: row r's operands are copied into one of
 // STAGES buffers by the bulk-copy engine while earlier rows are computed, so the
 // memory never waits for the arithmetic (with a CTA per row the two took turns:
-// SwiGLU of 2048 x 14336 bf16 40.6 us, against 22.4 of traffic).  A buffer is
+// SwiGLU of 2048 x 14336 bf16 40.6 us, now 35.0, against 22.4 of traffic).  A buffer is
 // free once the row's reduction has passed its barrier: every thread then holds
 // its values in registers.  LOOSE: rows of any base, stride and length, put back
 // on the grid from shared memory.  WTS_HELD: the norm weight is kept there too.
 template <typename XT, typename RT, int MODE, bool LOOSE, int C>
-__global__ void __launch_bounds__(kStreamThreads, C * 16 / (int)sizeof(XT) <= 32 ? 2 : 1) quantize_stream_kernel(const QuantRows Q, int stages, bool wts_held, int* err) {
+__global__ void __launch_bounds__(stream_threads(LOOSE), !LOOSE && C * 16 / (int)sizeof(XT) <= 32 ? 2 : 1)
+    quantize_stream_kernel(const QuantRows Q, int stages, bool wts_held, int* err) {
+    constexpr int kStreamThreads = stream_threads(LOOSE);
     constexpr int V = 16 / (int)sizeof(XT);
     extern __shared__ __align__(128) uint8_t sh[];
     uint64_t* full = reinterpret_cast<uint64_t*>(sh);
@@ -679,8 +688,8 @@ cudaError_t launch_stream(const QuantRows& q, int threads, int stages, bool wts_
 // rows that no buffer or no 64 values a thread hold.
 template <typename XT, typename RT, int MODE, bool LOOSE>
 cudaError_t try_stream(const QuantRows& q, cudaStream_t s) {
-    constexpr int V = 16 / (int)sizeof(XT);
-    if (q.k > 64 * kStreamThreads) return cudaErrorNotSupported;
+    constexpr int V = 16 / (int)sizeof(XT), kStreamThreads = stream_threads(LOOSE);
+    if (q.k > stream_values(LOOSE) * kStreamThreads) return cudaErrorNotSupported;
     const int64_t kv = (q.k + V - 1) / V * V;
     const bool two = MODE == kSwiglu || q.res;
     const size_t stage = staged_bytes(kv, sizeof(XT)) + (two ? staged_bytes(kv, sizeof(RT)) : 0u);
@@ -688,7 +697,7 @@ cudaError_t try_stream(const QuantRows& q, cudaStream_t s) {
     const int values = q.k <= 16 * kStreamThreads ? 16 : q.k <= 32 * kStreamThreads ? 32 : 64;  // a thread
     const int threads = (int)(((kv + values - 1) / values + 31) / 32 * 32);
     const auto room = [](int ctas) { return pipe::kSmemPerSm / (size_t)ctas - 1024 - kStreamHeader; };
-    const int at_once = values <= 32 ? 1024 : 512;  // threads that the registers leave room for
+    const int at_once = values <= 32 ? 1024 : 512;  // threads of an SM that the registers leave room for
     int ctas = at_once / threads < 8 ? at_once / threads : 8;
     if ((uintptr_t)q.norm_w % 16) wts = 0;  // the norm weight is held where a bulk copy can bring it
     while (ctas > 1 && room(ctas) < wts + 2 * stage) ctas--;
@@ -700,7 +709,9 @@ cudaError_t try_stream(const QuantRows& q, cudaStream_t s) {
     switch (values) {
     case 16: return launch_stream<XT, RT, MODE, LOOSE, 16 / V>(q, threads, stages, held, ctas, smem, s);
     case 32: return launch_stream<XT, RT, MODE, LOOSE, 32 / V>(q, threads, stages, held, ctas, smem, s);
-    default: return launch_stream<XT, RT, MODE, LOOSE, 64 / V>(q, threads, stages, held, ctas, smem, s);
+    default:
+        if constexpr (!LOOSE) return launch_stream<XT, RT, MODE, LOOSE, 64 / V>(q, threads, stages, held, ctas, smem, s);
+        return cudaErrorNotSupported;
     }
 }
 
@@ -730,7 +741,7 @@ cudaError_t launch_rows(const QuantRows& q, cudaStream_t s) {
 // Streams what is off the 16-byte grid, whose words only shared memory puts back
 // together (rows of at most 512 take a warp, an element at a time); and, of at
 // least four rows an SM, those whose arithmetic counts beside the traffic: 16-bit rows
-// (2048 x 14336 with an f32 residual and norm 59 us, a CTA per row 77; SwiGLU 36
+// (2048 x 14336 with an f32 residual and norm 60 us, a CTA per row 77; SwiGLU 35
 // and 41) and SwiGLU of long f32 ones (45 and 49).  f32 rows otherwise keep a CTA per
 // row (the norm 61 us, streamed 70).
 template <typename XT, typename RT, int MODE>

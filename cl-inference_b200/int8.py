@@ -145,10 +145,12 @@ class Int8Rows:
         if dtype is None:
             dtype = torch.float32 if out is None else out.dtype
         code = _type_code(dtype, "dtype")
-        if out is None:
-            out = codes.new_empty((m, k), dtype=dtype)
-        else:
+        if out is not None:
             _writable(out, "out", (m, k), dtype)
+        elif codes.is_contiguous():
+            out = torch.empty_like(codes, dtype=dtype)
+        else:
+            out = codes.new_empty((m, k), dtype=dtype)
         status = _lib_dequantize(codes.data_ptr(), _ld(codes, m, k), scales.data_ptr(), m, k, out.data_ptr(), code,
                                  _ld(out, m, k), _stream(device))
         if status:
@@ -161,8 +163,10 @@ def _empty_rows(x, m, k):
     boundaries, and their row stride."""
     q = Int8Rows.__new__(Int8Rows)
     pitch = (k + 15) // 16 * 16
-    codes = x.new_empty((m, pitch), dtype=_t.int8)
-    q.codes = codes if pitch == k else codes[:, :k]
+    if pitch == k and x.is_contiguous():
+        q.codes = _t.empty_like(x, dtype=_t.int8)
+    else:
+        q.codes = x.new_empty((m, pitch), dtype=_t.int8)[:, :k]
     q.scales = x.new_empty(m, dtype=_t.float32)
     return q, pitch
 
@@ -203,7 +207,7 @@ def norm_quantize(x, norm_weight=None, eps=1e-5, residual=None, residual_out=Non
         if rtype not in (xtype, _lib.CLQ_X_F32):
             raise ValueError(f"residual: {x.dtype} or float32, not {residual.dtype}")
         if residual_out is None:
-            residual_out = torch.empty_like(residual, memory_format=torch.contiguous_format)
+            residual_out = torch.empty_like(residual) if residual.is_contiguous() else residual.new_empty((m, k))
         else:
             _writable(residual_out, "residual_out", (m, k), residual.dtype)
             _apart(residual_out, given, "residual_out")

@@ -6,8 +6,9 @@ codes   before its rounding to a whole number a code is v * inv: v carries at mo
         roundings (residual sum, norm weight), peak / 127 and 1 / step one each, and the peak
         the two of its own v, the product one: 8 u relative of at most 127, so it is within
         127 * 8 u < 6.1e-5 of the exact quotient, and the code within 0.5 + 6.1e-5.
-        silu(g) * u adds expf (2 units in the last place: 4 u), 1 + e, the quotient and the product
-        (3 u), for v and for the peak: 127 * 22 u < 1.7e-4.
+        silu(g) * u comes from an exponential of 2^-22 (4 u), its argument's correction, 1 + e, a
+        reciprocal of 2^-23 (2 u) and two products (4 u): 10 u for v and 10 u for the peak, beside
+        the two of the step: 127 * 22 u < 1.7e-4.
 scales  peak / 127 and its product with s one rounding each beside the peak's own; the sum of k
         squares in some order of f32 additions in which no value passes more than k / 32 + 24
         of them, halved by the square root, which with the mean, the addition of eps, the square
