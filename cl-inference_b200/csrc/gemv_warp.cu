@@ -860,6 +860,7 @@ bool encode_rows(CUtensorMap* map, const void* base, int64_t rows, int64_t row_b
 
 bool encode_swizzled_rows(CUtensorMap* map, const void* base, int64_t rows, int64_t row_bytes, int64_t stride, int box_rows) {
     PFN_cuTensorMapEncodeTiled_v12000 fn = encode_tiled();
+    if (rows == 1) stride = (row_bytes + 15) / 16 * 16;  // a single row's is never used
     if (!fn || (uintptr_t)base % 16 || stride % 16 || rows < 1 || row_bytes < 1 || box_rows < 1 || box_rows > 256)
         return false;
     const cuuint64_t dims[2] = {(cuuint64_t)row_bytes, (cuuint64_t)rows};

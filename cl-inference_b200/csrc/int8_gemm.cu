@@ -212,6 +212,7 @@ __device__ __forceinline__ void emit_columns(const Int8Product& p, const int (&v
 #pragma unroll
     for (int j = 0; j < 32; j++, out += p.ldo)
         if (j < cnt) *out = int8_round<OT>(o[j]);
+    __syncwarp();  // the next tensor-memory load wants the whole warp
 }
 template <typename OT>
 __device__ __forceinline__ void emit32(const Int8Product& p, const int (&v)[32], int64_t n, float wsn, int64_t t0, int cnt,
@@ -406,6 +407,7 @@ __global__ void __launch_bounds__(kThreads) int8_tile_kernel(const __grid_consta
                 for (int j = 0; j < 32; j++) sums[(c + j) * kRows + 32 * warp + lane] = v[j];
             }
         }
+        __syncwarp();
         cluster_arrive();
         cluster_wait();
         if (ok) {
@@ -429,6 +431,7 @@ __global__ void __launch_bounds__(kThreads) int8_tile_kernel(const __grid_consta
                 }
             }
         }
+        __syncwarp();
         cluster_arrive();
         cluster_wait();  // the other parts have read this CTA's sums
     }

@@ -5,21 +5,14 @@
 // choice of a kernel, and the kernel for operands that no wide load can read.
 #include <cstdint>
 
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
 #include "../../include/clq.h"
 #include "clq_internal.h"
+#include "int8_out.cuh"
 
 namespace clq {
 namespace {
-
-__device__ __forceinline__ void store_out(void* out, int otype, int64_t i, float v) {
-    if (otype == CLQ_X_F32) static_cast<float*>(out)[i] = v;
-    else if (otype == CLQ_X_BF16) static_cast<__nv_bfloat16*>(out)[i] = __float2bfloat16_rn(v);
-    else static_cast<__half*>(out)[i] = __float2half_rn(v);
-}
 
 // A CTA forms 64 x 64 outputs, 4 x 4 a thread, from 32-byte columns of both
 // operands staged in shared memory a byte at a time (any base and stride),
@@ -27,44 +20,48 @@ __device__ __forceinline__ void store_out(void* out, int otype, int64_t i, float
 constexpr int kGT = 64, kGK = 32;
 __global__ void __launch_bounds__(256) linear_int8_generic_kernel(const Int8Product P) {
     __shared__ int xs[kGK / 4][kGT + 1], ws[kGK / 4][kGT + 1];
-    const int64_t t0 = (int64_t)blockIdx.y * kGT, n0 = (int64_t)blockIdx.x * kGT;
+    const int64_t n0 = (int64_t)blockIdx.x * kGT;
     const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-    int acc[4][4] = {};
-    for (int64_t k0 = 0; k0 < P.k; k0 += kGK) {
-        for (int e = threadIdx.x; e < kGT * kGK / 4; e += 256) {
-            const int r = e / (kGK / 4), c = e % (kGK / 4);
-            uint32_t a = 0, b = 0;
-            for (int i = 0; i < 4; i++) {
-                const int64_t kk = k0 + 4 * c + i;
-                if (kk < P.k && t0 + r < P.m) a |= (uint32_t)(uint8_t)P.x[(t0 + r) * P.ldx + kk] << (8 * i);
-                if (kk < P.k && n0 + r < P.n) b |= (uint32_t)(uint8_t)P.w[(n0 + r) * P.ldw + kk] << (8 * i);
+    for (int64_t t0 = (int64_t)blockIdx.y * kGT; t0 < P.m; t0 += (int64_t)gridDim.y * kGT) {
+        int acc[4][4] = {};
+        for (int64_t k0 = 0; k0 < P.k; k0 += kGK) {
+            for (int e = threadIdx.x; e < kGT * kGK / 4; e += 256) {
+                const int r = e / (kGK / 4), c = e % (kGK / 4);
+                uint32_t a = 0, b = 0;
+                for (int i = 0; i < 4; i++) {
+                    const int64_t kk = k0 + 4 * c + i;
+                    if (kk < P.k && t0 + r < P.m) a |= (uint32_t)(uint8_t)P.x[(t0 + r) * P.ldx + kk] << (8 * i);
+                    if (kk < P.k && n0 + r < P.n) b |= (uint32_t)(uint8_t)P.w[(n0 + r) * P.ldw + kk] << (8 * i);
+                }
+                xs[c][r] = (int)a;
+                ws[c][r] = (int)b;
             }
-            xs[c][r] = (int)a;
-            ws[c][r] = (int)b;
+            __syncthreads();
+#pragma unroll
+            for (int c = 0; c < kGK / 4; c++)
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++) acc[i][j] = __dp4a(xs[c][ty + 16 * i], ws[c][tx + 16 * j], acc[i][j]);
+            __syncthreads();
         }
-        __syncthreads();
-#pragma unroll
-        for (int c = 0; c < kGK / 4; c++)
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-#pragma unroll
-                for (int j = 0; j < 4; j++) acc[i][j] = __dp4a(xs[c][ty + 16 * i], ws[c][tx + 16 * j], acc[i][j]);
-        __syncthreads();
+        for (int i = 0; i < 4; i++)
+            for (int j = 0; j < 4; j++) {
+                const int64_t t = t0 + ty + 16 * i, n = n0 + tx + 16 * j;
+                if (t >= P.m || n >= P.n) continue;
+                float v = int8_scaled(acc[i][j], P.ws[n], P.xs[t]);
+                if (P.res) v = __fadd_rn(v, P.res[t * P.ldr + n]);
+                if (P.otype == CLQ_X_F32) static_cast<float*>(P.out)[t * P.ldo + n] = v;
+                else if (P.otype == CLQ_X_BF16) static_cast<__nv_bfloat16*>(P.out)[t * P.ldo + n] = int8_round<__nv_bfloat16>(v);
+                else static_cast<__half*>(P.out)[t * P.ldo + n] = int8_round<__half>(v);
+            }
     }
-    for (int i = 0; i < 4; i++)
-        for (int j = 0; j < 4; j++) {
-            const int64_t t = t0 + ty + 16 * i, n = n0 + tx + 16 * j;
-            if (t >= P.m || n >= P.n) continue;
-            float v = __fmul_rn(__fmul_rn((float)acc[i][j], P.ws[n]), P.xs[t]);
-            if (P.res) v = __fadd_rn(v, P.res[t * P.ldr + n]);
-            store_out(P.out, P.otype, t * P.ldo + n, v);
-        }
 }
 
 cudaError_t launch_linear_int8_generic(const Int8Product& p, cudaStream_t s) {
     const int64_t bx = (p.n + kGT - 1) / kGT, by = (p.m + kGT - 1) / kGT;
-    if (by > 65535 || bx > INT32_MAX) return cudaErrorInvalidConfiguration;
-    linear_int8_generic_kernel<<<dim3((unsigned)bx, (unsigned)by), 256, 0, s>>>(p);
+    if (bx > INT32_MAX || by > INT32_MAX) return cudaErrorInvalidConfiguration;
+    linear_int8_generic_kernel<<<dim3((unsigned)bx, (unsigned)(by < 65535 ? by : 65535)), 256, 0, s>>>(p);
     return cudaGetLastError();
 }
 
@@ -129,6 +126,10 @@ int clq_norm_quantize_device(const void* x, int xtype, int64_t m, int64_t k, int
         return clq::set_error(CLQ_ERR_SHAPE, "residual output stride %lld below the row length %lld", (long long)ldro,
                               (long long)k);
     if (norm_weight && !(norm_epsilon >= 0.f)) return i8_fail(CLQ_ERR_ARGUMENT, "the norm's epsilon must not be negative");
+    if (residual_out && residual_out == residual && m > 1 && ldro != ldr)
+        return i8_fail(CLQ_ERR_SHAPE, "the residual and its output are one matrix with two row strides");
+    if (residual_out && residual_out == x && (rtype != xtype || (m > 1 && ldro != ldx)))
+        return i8_fail(CLQ_ERR_SHAPE, "the rows and the residual's output are one matrix with two layouts");
     clq::QuantRows q = {};
     q.x = x;
     q.xtype = xtype;
@@ -194,6 +195,8 @@ int clq_linear_int8_device(const int8_t* x, int64_t ldx, const float* x_scales, 
         return clq::set_error(CLQ_ERR_UNSUPPORTED, "rows of %lld codes (32-bit sums hold %d)", (long long)k, CLQ_INT8_MAX_K);
     if (m > 1 && (ldo < n || (residual && ldr < n)))
         return clq::set_error(CLQ_ERR_SHAPE, "output or residual stride below %lld columns", (long long)n);
+    if (residual && residual == out && (otype != CLQ_X_F32 || (m > 1 && ldr != ldo)))
+        return i8_fail(CLQ_ERR_SHAPE, "the residual and the output are one matrix with two layouts");
     if (m == 0 || n == 0) return CLQ_OK;
     if (!out || !x_scales || !w_scales || (k > 0 && (!x || !w))) return i8_fail(CLQ_ERR_ARGUMENT, "null operand or output");
     if ((rc = clq::sm100_device(&dev))) return rc;

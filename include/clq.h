@@ -350,11 +350,11 @@ int clq_attend_device(const float *q, int64_t count, int n_heads, int64_t q_pos_
 /* M rows of K elements of XTYPE (clq_xtype). */
 int clq_quantize_rows_device(const void *x, int xtype, int64_t m, int64_t k, int64_t ldx, int8_t *codes,
                              int64_t ldc, float *scales, void *stream);
-/* h = x + residual, rounded into RESIDUAL_OUT; the codes are those of the f32
+/* h = x + residual, rounded into RESIDUAL_OUT (which may be RESIDUAL, or X of RTYPE,
+ * with its stride); the codes are those of the f32
  * h * norm_weight and the scales those times 1 / sqrt(mean(h^2) + norm_epsilon)
  * (the residual addition of layer-forward, local/blocks.lisp:387-392, and the
- * apply-rmsnorm of the next block, :115-116).  RESIDUAL, RESIDUAL_OUT (which may
- * be RESIDUAL) and NORM_WEIGHT (f32 [K]; without it h itself is coded) may be
+ * apply-rmsnorm of the next block, :115-116).  RESIDUAL, RESIDUAL_OUT and NORM_WEIGHT (f32 [K]; without it h itself is coded) may be
  * null.  RTYPE, of both residuals, is XTYPE or CLQ_X_F32.  A row whose sum of
  * squares leaves f32 counts as non-finite. */
 int clq_norm_quantize_device(const void *x, int xtype, int64_t m, int64_t k, int64_t ldx, const float *norm_weight,
@@ -369,7 +369,8 @@ int clq_dequantize_rows_device(const int8_t *codes, int64_t ldc, const float *sc
 /* out[t, j] = sum_c x[t, c] w[j, c] * w_scales[j] * x_scales[t] (+ residual[t, j]) for
  * M token rows and N channel rows of K codes (any int8 value), rounded once to OTYPE: the
  * linear of local/blocks.lisp:106-113 with both operands in 8 bits.  The sum is an
- * exact 32-bit integer, which bounds K.  RESIDUAL (f32) may be null, or OUT itself. */
+ * exact 32-bit integer, which bounds K.  RESIDUAL (f32) may be null, or an f32 OUT
+ * itself (with its stride). */
 #define CLQ_INT8_MAX_K 131071
 int clq_linear_int8_device(const int8_t *x, int64_t ldx, const float *x_scales, int64_t m, const int8_t *w,
                            int64_t ldw, const float *w_scales, int64_t n, int64_t k, const float *residual,

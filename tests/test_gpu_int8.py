@@ -303,7 +303,8 @@ def test_linear_over_weights(cuda, clq, m, n, k):
 
 
 @pytest.mark.parametrize("m,n,k", [(2048, 4096, 4096), (1, 28672, 4096), (16, 4096, 14336), (1500, 3000, 700),
-                                   (4096, 1024, 512), (8, 128256, 256)])
+                                   (4096, 1024, 512), (8, 128256, 256), (250, 19200, 4096), (300, 4864, 2048),
+                                   (1111, 9472, 1024), (77, 512, 40000)])
 def test_linear_at_size(cuda, clq, m, n, k):
     torch = cuda
     w = clq.Int8Rows(*codes_of(torch, n, k, seed=n + k))
@@ -493,6 +494,8 @@ def test_a_stream_by_handle(cuda, clq):
     w = clq.quantize_rows(rand(torch, 256, 4096, seed=2))
     want = clq.linear_int8(clq.quantize_rows(x), w)
     torch.cuda.synchronize()
+    default = torch.cuda.default_stream().cuda_stream
+    assert torch.equal(clq.linear_int8(clq.quantize_rows(x, stream=default), w, stream=default), want)
     h = side.cuda_stream
     for _ in range(20):
         with torch.cuda.stream(side):

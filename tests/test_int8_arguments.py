@@ -33,6 +33,9 @@ def test_norm_quantizer_checks_its_residual(clq):
     assert call(ldro=7) == 2
     assert call(eps=-1.0) == 1
     assert call(eps=float("nan")) == 1
+    assert c(clq, "clq_norm_quantize_device", 512, 0, 2, 8, 8, None, 0.0, FAKE, 0, 16, FAKE, 8, FAKE, 8, FAKE, None) == 2
+    assert "two row strides" in clq._lib.last_error()  # in place, but not on itself
+    assert c(clq, "clq_norm_quantize_device", FAKE, 1, 2, 8, 8, None, 0.0, 512, 0, 8, FAKE, 8, FAKE, 8, FAKE, None) == 2
 
 
 def test_swiglu_and_dequantize_check_arguments(clq):
@@ -57,6 +60,8 @@ def test_product_checks_arguments(clq):
     assert call(ldw=63) == 2
     assert call(ldo=2) == 2
     assert call(res=FAKE, ldr=2) == 2
+    assert call(res=FAKE, ldr=4) == 2                         # onto the output, with another stride
+    assert call(res=FAKE, ldr=3, otype=1) == 2                # or of another type
     assert call(k=131072, ldx=131072, ldw=131072) == 9        # 32-bit sums could wrap
     assert "131071" in clq._lib.last_error()
     for missing in ("x", "xs", "w", "ws", "out"):
