@@ -183,6 +183,21 @@ __device__ __forceinline__ bool wait_spin(uint64_t* bar, uint32_t parity, int* e
     if (i == kWaitLimit) atomicExch(err, CLQ_ERR_TIMEOUT);
     return __all_sync(0xffffffffu, ok);
 }
+// A role's place in a ring of N stages: the stage and the parity of its round.
+// Stepped rather than divided out of a count: the loops' rate is that of one
+// warp's instructions (a division a stage cost 0.1 us of 0.28).
+template <int N>
+struct Ring {
+    int s = 0;
+    uint32_t round = 0;
+    __device__ __forceinline__ void next() {
+        if (++s == N) {
+            s = 0;
+            round++;
+        }
+    }
+    __device__ __forceinline__ uint32_t parity() const { return round & 1u; }
+};
 __device__ __forceinline__ uint8_t* align1024(uint8_t* p) {
     return reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(p) + 1023) & ~(uintptr_t)1023);
 }
@@ -343,14 +358,14 @@ __global__ void __launch_bounds__(kThreads) int8_tile_kernel(const __grid_consta
 
     bool ok = false;
     if (warp == 4) {
+        Ring<NS> r;
         int it = 0;
-        for (; it < nk; it++) {
-            const int s = it % NS;
-            if (it >= NS && !wait_spin(&empty[s], ((it / NS) - 1) & 1, G.err)) break;
+        for (; it < nk; it++, r.next()) {
+            if (r.round && !wait_spin(&empty[r.s], r.parity() ^ 1u, G.err)) break;
             if (elect_one()) {
-                mbar_arrive_tx(&full[s], kABytes + kBBytes);
-                tensor_copy_2d(A + (size_t)s * kABytes, &G.wmap, (kb0 + it) * kKB, (int)n0, &full[s]);
-                tensor_copy_2d(B + (size_t)s * kBBytes, &G.xmap, (kb0 + it) * kKB, (int)t0, &full[s]);
+                mbar_arrive_tx(&full[r.s], kABytes + kBBytes);
+                tensor_copy_2d(A + (size_t)r.s * kABytes, &G.wmap, (kb0 + it) * kKB, (int)n0, &full[r.s]);
+                tensor_copy_2d(B + (size_t)r.s * kBBytes, &G.xmap, (kb0 + it) * kKB, (int)t0, &full[r.s]);
             }
             __syncwarp();
         }
@@ -358,16 +373,16 @@ __global__ void __launch_bounds__(kThreads) int8_tile_kernel(const __grid_consta
         for (int i = it < NS ? 0 : it - NS; i < it; i++) mbar_drain(&full[i % NS], (i / NS) & 1);
     } else if (warp == 5) {
         constexpr uint32_t idesc = instr_desc_i8(kRows, TN);
-        for (int it = 0; it < nk; it++) {
-            const int s = it % NS;
-            if (!wait_spin(&full[s], (it / NS) & 1, G.err)) break;
+        Ring<NS> r;
+        for (int it = 0; it < nk; it++, r.next()) {
+            if (!wait_spin(&full[r.s], r.parity(), G.err)) break;
             tc_fence_after();
-            const uint32_t a = smem_u32(A + (size_t)s * kABytes), b = smem_u32(B + (size_t)s * kBBytes);
+            const uint32_t a = smem_u32(A + (size_t)r.s * kABytes), b = smem_u32(B + (size_t)r.s * kBBytes);
             if (elect_one()) {
 #pragma unroll
                 for (int j = 0; j < kKB / 32; j++)
                     mma_i8<1>(tmem, smem_desc(a + 32 * j), smem_desc(b + 32 * j), idesc, it > 0 || j > 0);
-                mma_commit<1>(&empty[s]);
+                mma_commit<1>(&empty[r.s]);
             }
             __syncwarp();
         }
@@ -511,7 +526,7 @@ __global__ void __launch_bounds__(kThreads, 1) int8_pair_kernel(const __grid_con
     allow_dependents();
 
     if (warp == 4) {
-        int64_t it = 0;
+        Ring<NS> r;
         bool ok = true;
         for (int64_t tile = first; tile < tiles && ok; tile += step) {
             const PairUnit u = pair_unit(G, tile);
@@ -519,27 +534,27 @@ __global__ void __launch_bounds__(kThreads, 1) int8_pair_kernel(const __grid_con
             const int y_w = (int)(u.rt * 2 * kRows + rank * kRows), y_x = (int)(u.t0 + rank * (u.tokens / 2));
             const CUtensorMap* xmap = u.tokens == kPairTokens ? &G.xmap : &G.xmap_part;
             const uint32_t tx = 2u * (kABytes + (uint32_t)u.tokens / 2 * kKB);
-            for (int kb = 0; kb < nk; kb++, it++) {
-                const int s = (int)(it % NS);
-                if (it >= NS && !(ok = wait_spin(&empty[s], (uint32_t)((it / NS) - 1) & 1u, G.err))) break;
+            for (int kb = 0; kb < nk; kb++, r.next()) {
+                if (r.round && !(ok = wait_spin(&empty[r.s], r.parity() ^ 1u, G.err))) break;
                 if (elect_one()) {
-                    if (leader) mbar_arrive_tx(&full[s], tx);
-                    const uint32_t bar = map_rank(smem_u32(&full[s]), 0);
-                    tensor_copy_pair(A + (size_t)s * kABytes, &G.wmap, kb * kKB, y_w, bar);
-                    tensor_copy_pair(B + (size_t)s * kPairB, xmap, kb * kKB, y_x, bar);
+                    if (leader) mbar_arrive_tx(&full[r.s], tx);
+                    const uint32_t bar = map_rank(smem_u32(&full[r.s]), 0);
+                    tensor_copy_pair(A + (size_t)r.s * kABytes, &G.wmap, kb * kKB, y_w, bar);
+                    tensor_copy_pair(B + (size_t)r.s * kPairB, xmap, kb * kKB, y_x, bar);
                 }
                 __syncwarp();
             }
         }
         // every stage has been read, and the leader's commits have arrived here, before the CTA exits
-        for (int64_t i = it < NS ? 0 : it - NS; i < it && ok; i++)
-            ok = wait_spin(&empty[i % NS], (uint32_t)(i / NS) & 1u, G.err);
+        for (int i = 0; i < NS && ok; i++, r.next())
+            if (r.round) ok = wait_spin(&empty[r.s], r.parity() ^ 1u, G.err);
         // after a wait that gave up, the copies in flight (their barrier may be the other CTA's) get
         // 100 us to land: a hundred times what one takes
         for (int i = 0; i < 100 && !ok; i++) __nanosleep(1000);
     } else if (warp == 5) {
         if (leader) {
-            int64_t it = 0, nt = 0;
+            Ring<NS> r;
+            int64_t nt = 0;
             bool ok = true;
             for (int64_t tile = first; tile < tiles && ok; tile += step, nt++) {
                 const PairUnit u = pair_unit(G, tile);
@@ -548,17 +563,16 @@ __global__ void __launch_bounds__(kThreads, 1) int8_pair_kernel(const __grid_con
                 const int buf = (int)(nt & 1);
                 if (nt >= 2 && !(ok = wait_spin(&acc_empty[buf], (uint32_t)((nt >> 1) - 1) & 1u, G.err))) break;
                 tc_fence_after();
-                for (int kb = 0; kb < nk; kb++, it++) {
-                    const int s = (int)(it % NS);
-                    if (!(ok = wait_spin(&full[s], (uint32_t)(it / NS) & 1u, G.err))) break;
+                for (int kb = 0; kb < nk; kb++, r.next()) {
+                    if (!(ok = wait_spin(&full[r.s], r.parity(), G.err))) break;
                     tc_fence_after();
-                    const uint32_t a = smem_u32(A + (size_t)s * kABytes), b = smem_u32(B + (size_t)s * kPairB);
+                    const uint32_t a = smem_u32(A + (size_t)r.s * kABytes), b = smem_u32(B + (size_t)r.s * kPairB);
                     if (elect_one()) {
 #pragma unroll
                         for (int j = 0; j < kKB / 32; j++)
                             mma_i8<2>(tmem + (uint32_t)(buf * kPairTokens), smem_desc(a + 32 * j), smem_desc(b + 32 * j),
                                       idesc, kb > 0 || j > 0);
-                        mma_commit<2>(&empty[s]);
+                        mma_commit<2>(&empty[r.s]);
                     }
                     __syncwarp();
                 }
