@@ -80,41 +80,46 @@ __device__ __forceinline__ int4 load_cluster(uint32_t addr) {
 __device__ __forceinline__ void arrive_cluster(uint32_t bar) {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
-// K-major, SWIZZLE_128B, 8-row groups 1024 bytes apart.
-__device__ __forceinline__ uint64_t smem_desc(uint32_t addr) {
-    return (uint64_t)((addr >> 4) & 0x3FFF) | ((uint64_t)1 << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) |
-           ((uint64_t)2 << 61);
-}
 // Signed 8-bit A and B (K-major), 32-bit integer D, M x N.
 __host__ __device__ constexpr uint32_t instr_desc_i8(int m, int n) {
     return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
+// Low word of the matrix descriptor of an operand at shared ADDR (under 256 KB);
+// the high word is the same for all: K-major, SWIZZLE_128B, 8-row groups 1024
+// bytes apart.
+__device__ __forceinline__ uint32_t desc_low(uint32_t addr) { return (addr >> 4) | (1u << 16); }
+constexpr uint32_t kDescHigh = (1024u >> 4) | (1u << 14) | (2u << 29);
+#define CLQ_MMA_STAGE(CG)                                                                                            \
+    "{\n\t.reg .pred p, q;\n\t.reg .b64 da, db;\n\t.reg .b32 x, y;\n\t"                                             \
+    "setp.ne.b32 p, %4, 0;\n\tsetp.eq.b32 q, %5, %5;\n\t"                                                            \
+    "mov.b64 da, {%1, %5};\n\tmov.b64 db, {%2, %5};\n\t"                                                             \
+    "tcgen05.mma.cta_group::" CG ".kind::i8 [%0], da, db, %3, p;\n\t"                                                \
+    "add.u32 x, %1, 2;\n\tadd.u32 y, %2, 2;\n\tmov.b64 da, {x, %5};\n\tmov.b64 db, {y, %5};\n\t"                    \
+    "tcgen05.mma.cta_group::" CG ".kind::i8 [%0], da, db, %3, q;\n\t"                                                \
+    "add.u32 x, %1, 4;\n\tadd.u32 y, %2, 4;\n\tmov.b64 da, {x, %5};\n\tmov.b64 db, {y, %5};\n\t"                    \
+    "tcgen05.mma.cta_group::" CG ".kind::i8 [%0], da, db, %3, q;\n\t"                                                \
+    "add.u32 x, %1, 6;\n\tadd.u32 y, %2, 6;\n\tmov.b64 da, {x, %5};\n\tmov.b64 db, {y, %5};\n\t"                    \
+    "tcgen05.mma.cta_group::" CG ".kind::i8 [%0], da, db, %3, q;\n\t}"
+// The four MMAs (32 codes of K each) of one stage; A, B: low descriptor words.
+// ACCUMULATE 0: the first of them overwrites the accumulator.
 template <int CG>
-__device__ __forceinline__ void mma_i8(uint32_t tmem, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+__device__ __forceinline__ void mma_stage(uint32_t tmem, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
+    static_assert(kKB == 128, "four MMAs to a stage");
     if constexpr (CG == 1)
-        asm volatile(
-            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-            "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem),
-            "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
-            : "memory");
+        asm volatile(CLQ_MMA_STAGE("1") ::"r"(tmem), "r"(a), "r"(b), "r"(idesc), "r"(accumulate), "r"(kDescHigh) : "memory");
     else
-        asm volatile(
-            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-            "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem),
-            "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
-            : "memory");
+        asm volatile(CLQ_MMA_STAGE("2") ::"r"(tmem), "r"(a), "r"(b), "r"(idesc), "r"(accumulate), "r"(kDescHigh) : "memory");
 }
+#undef CLQ_MMA_STAGE
 // Arrives on BAR once every MMA issued before has completed; CG 2: on the
 // barriers at BAR's offset in both CTAs of the pair.
 template <int CG>
-__device__ __forceinline__ void mma_commit(uint64_t* bar) {
+__device__ __forceinline__ void mma_commit(uint32_t bar) {
     if constexpr (CG == 1)
-        asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
-                     : "memory");
+        asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
     else
         asm volatile(
-            "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
-                smem_u32(bar)),
+            "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
             "h"((uint16_t)3)
             : "memory");
 }
@@ -152,14 +157,46 @@ __device__ __forceinline__ void tmem_load32(uint32_t addr, int (&v)[32]) {
 __device__ __forceinline__ void prefetch_map(const void* map) {
     asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
 }
-// A box of MAP at (X bytes, row Y) into this CTA's DST, counted on BAR, a
-// shared::cluster address that may lie in the pair's other CTA.
-__device__ __forceinline__ void tensor_copy_pair(void* dst, const void* map, int x, int y, uint32_t bar) {
+// The loops that issue copies and MMAs run at the rate of one warp's
+// instructions, so they work on 32-bit shared addresses throughout.
+//
+// A box of MAP at (X bytes, row Y) into this CTA's DST, counted on BAR; CG 2: BAR
+// may lie in the pair's other CTA (a shared::cluster address).
+template <int CG>
+__device__ __forceinline__ void copy_box(uint32_t dst, const void* map, int x, int y, uint32_t bar) {
+    if constexpr (CG == 1)
+        asm volatile(
+            "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+            "l"(map), "r"(x), "r"(y), "r"(bar)
+            : "memory");
+    else
+        asm volatile(
+            "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], "
+            "[%4];" ::"r"(dst),
+            "l"(map), "r"(x), "r"(y), "r"(bar)
+            : "memory");
+}
+__device__ __forceinline__ void arrive_tx(uint32_t bar, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+// Whether the phase has completed: at once, or after the pause that try_wait may take.
+__device__ __forceinline__ bool peek(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
     asm volatile(
-        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], "
-        "[%4];" ::"r"(smem_u32(dst)),
-        "l"(map), "r"(x), "r"(y), "r"(bar)
+        "{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
         : "memory");
+    return ok != 0;
+}
+__device__ __forceinline__ bool test(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    return ok != 0;
 }
 // One lane of a converged warp.  The copying and the issuing warp run their
 // loops as whole warps and elect a lane around the asynchronous instructions
@@ -172,12 +209,14 @@ __device__ __forceinline__ bool elect_one() {
     return e != 0;
 }
 // Bounded wait of a whole warp that spins without sleeping (a stage is a few
-// hundred cycles); every lane gets the same answer.
-__device__ __forceinline__ bool wait_spin(uint64_t* bar, uint32_t parity, int* err) {
+// hundred cycles); every lane gets the same answer.  READY: what a peek at the
+// barrier, made while other work was under way, found.
+__device__ __forceinline__ bool wait_spin(uint32_t bar, uint32_t parity, int* err, bool ready = false) {
+    if (__all_sync(0xffffffffu, ready)) return true;
     bool ok = false;
     uint32_t i = 0;
     for (; i < kWaitLimit; i++) {
-        if ((ok = mbar_test(bar, parity))) break;
+        if ((ok = test(bar, parity))) break;
         if ((i & 1023) == 1023 && *(volatile int*)err) break;
     }
     if (i == kWaitLimit) atomicExch(err, CLQ_ERR_TIMEOUT);
@@ -197,6 +236,11 @@ struct Ring {
         }
     }
     __device__ __forceinline__ uint32_t parity() const { return round & 1u; }
+    __device__ __forceinline__ Ring after() const {
+        Ring r = *this;
+        r.next();
+        return r;
+    }
 };
 __device__ __forceinline__ uint8_t* align1024(uint8_t* p) {
     return reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(p) + 1023) & ~(uintptr_t)1023);
@@ -357,36 +401,42 @@ __global__ void __launch_bounds__(kThreads) int8_tile_kernel(const __grid_consta
     allow_dependents();
 
     bool ok = false;
+    const uint32_t fulls = smem_u32(full), empties = smem_u32(empty);
     if (warp == 4) {
+        const uint32_t a0 = smem_u32(A), b0 = smem_u32(B);
         Ring<NS> r;
         int it = 0;
+        bool ready = false;
         for (; it < nk; it++, r.next()) {
-            if (r.round && !wait_spin(&empty[r.s], r.parity() ^ 1u, G.err)) break;
+            if (r.round && !wait_spin(empties + 8 * r.s, r.parity() ^ 1u, G.err, ready)) break;
+            const Ring<NS> next = r.after();
+            ready = next.round && peek(empties + 8 * next.s, next.parity() ^ 1u);
             if (elect_one()) {
-                mbar_arrive_tx(&full[r.s], kABytes + kBBytes);
-                tensor_copy_2d(A + (size_t)r.s * kABytes, &G.wmap, (kb0 + it) * kKB, (int)n0, &full[r.s]);
-                tensor_copy_2d(B + (size_t)r.s * kBBytes, &G.xmap, (kb0 + it) * kKB, (int)t0, &full[r.s]);
+                arrive_tx(fulls + 8 * r.s, kABytes + kBBytes);
+                copy_box<1>(a0 + r.s * kABytes, &G.wmap, (kb0 + it) * kKB, (int)n0, fulls + 8 * r.s);
+                copy_box<1>(b0 + r.s * kBBytes, &G.xmap, (kb0 + it) * kKB, (int)t0, fulls + 8 * r.s);
             }
             __syncwarp();
         }
         // what is in flight lands before the CTA exits
         for (int i = it < NS ? 0 : it - NS; i < it; i++) mbar_drain(&full[i % NS], (i / NS) & 1);
     } else if (warp == 5) {
+        const uint32_t a0 = desc_low(smem_u32(A)), b0 = desc_low(smem_u32(B));
         constexpr uint32_t idesc = instr_desc_i8(kRows, TN);
         Ring<NS> r;
+        bool ready = false;
         for (int it = 0; it < nk; it++, r.next()) {
-            if (!wait_spin(&full[r.s], r.parity(), G.err)) break;
+            if (!wait_spin(fulls + 8 * r.s, r.parity(), G.err, ready)) break;
+            const Ring<NS> next = r.after();
+            ready = peek(fulls + 8 * next.s, next.parity());
             tc_fence_after();
-            const uint32_t a = smem_u32(A + (size_t)r.s * kABytes), b = smem_u32(B + (size_t)r.s * kBBytes);
             if (elect_one()) {
-#pragma unroll
-                for (int j = 0; j < kKB / 32; j++)
-                    mma_i8<1>(tmem, smem_desc(a + 32 * j), smem_desc(b + 32 * j), idesc, it > 0 || j > 0);
-                mma_commit<1>(&empty[r.s]);
+                mma_stage<1>(tmem, a0 + r.s * (kABytes >> 4), b0 + r.s * (kBBytes >> 4), idesc, it > 0);
+                mma_commit<1>(empties + 8 * r.s);
             }
             __syncwarp();
         }
-        if (elect_one()) mma_commit<1>(done);
+        if (elect_one()) mma_commit<1>(smem_u32(done));
         __syncwarp();
         mbar_drain(done, 0);
     } else {
@@ -525,9 +575,11 @@ __global__ void __launch_bounds__(kThreads, 1) int8_pair_kernel(const __grid_con
     grid_dependency_wait();
     allow_dependents();
 
+    const uint32_t fulls = smem_u32(full), empties = smem_u32(empty);
     if (warp == 4) {
+        const uint32_t a0 = smem_u32(A), b0 = smem_u32(B), fulls_leader = map_rank(fulls, 0);
         Ring<NS> r;
-        bool ok = true;
+        bool ok = true, ready = false;
         for (int64_t tile = first; tile < tiles && ok; tile += step) {
             const PairUnit u = pair_unit(G, tile);
             if (u.t0 >= P.m) break;  // a part past the last token, which is a CTA's last unit
@@ -535,48 +587,48 @@ __global__ void __launch_bounds__(kThreads, 1) int8_pair_kernel(const __grid_con
             const CUtensorMap* xmap = u.tokens == kPairTokens ? &G.xmap : &G.xmap_part;
             const uint32_t tx = 2u * (kABytes + (uint32_t)u.tokens / 2 * kKB);
             for (int kb = 0; kb < nk; kb++, r.next()) {
-                if (r.round && !(ok = wait_spin(&empty[r.s], r.parity() ^ 1u, G.err))) break;
+                if (r.round && !(ok = wait_spin(empties + 8 * r.s, r.parity() ^ 1u, G.err, ready))) break;
+                const Ring<NS> next = r.after();
+                ready = next.round && peek(empties + 8 * next.s, next.parity() ^ 1u);
                 if (elect_one()) {
-                    if (leader) mbar_arrive_tx(&full[r.s], tx);
-                    const uint32_t bar = map_rank(smem_u32(&full[r.s]), 0);
-                    tensor_copy_pair(A + (size_t)r.s * kABytes, &G.wmap, kb * kKB, y_w, bar);
-                    tensor_copy_pair(B + (size_t)r.s * kPairB, xmap, kb * kKB, y_x, bar);
+                    if (leader) arrive_tx(fulls + 8 * r.s, tx);
+                    copy_box<2>(a0 + r.s * kABytes, &G.wmap, kb * kKB, y_w, fulls_leader + 8 * r.s);
+                    copy_box<2>(b0 + r.s * kPairB, xmap, kb * kKB, y_x, fulls_leader + 8 * r.s);
                 }
                 __syncwarp();
             }
         }
         // every stage has been read, and the leader's commits have arrived here, before the CTA exits
         for (int i = 0; i < NS && ok; i++, r.next())
-            if (r.round) ok = wait_spin(&empty[r.s], r.parity() ^ 1u, G.err);
+            if (r.round) ok = wait_spin(empties + 8 * r.s, r.parity() ^ 1u, G.err);
         // after a wait that gave up, the copies in flight (their barrier may be the other CTA's) get
         // 100 us to land: a hundred times what one takes
         for (int i = 0; i < 100 && !ok; i++) __nanosleep(1000);
     } else if (warp == 5) {
         if (leader) {
+            const uint32_t a0 = desc_low(smem_u32(A)), b0 = desc_low(smem_u32(B)), accs = smem_u32(acc_full);
             Ring<NS> r;
             int64_t nt = 0;
-            bool ok = true;
+            bool ok = true, ready = false;
             for (int64_t tile = first; tile < tiles && ok; tile += step, nt++) {
                 const PairUnit u = pair_unit(G, tile);
                 if (u.t0 >= P.m) break;
                 const uint32_t idesc = instr_desc_i8(2 * kRows, u.tokens);
-                const int buf = (int)(nt & 1);
-                if (nt >= 2 && !(ok = wait_spin(&acc_empty[buf], (uint32_t)((nt >> 1) - 1) & 1u, G.err))) break;
+                const uint32_t buf = (uint32_t)(nt & 1), acc = tmem + buf * kPairTokens;
+                if (nt >= 2 && !(ok = wait_spin(smem_u32(acc_empty) + 8 * buf, (uint32_t)((nt >> 1) - 1) & 1u, G.err))) break;
                 tc_fence_after();
                 for (int kb = 0; kb < nk; kb++, r.next()) {
-                    if (!(ok = wait_spin(&full[r.s], r.parity(), G.err))) break;
+                    if (!(ok = wait_spin(fulls + 8 * r.s, r.parity(), G.err, ready))) break;
+                    const Ring<NS> next = r.after();
+                    ready = peek(fulls + 8 * next.s, next.parity());
                     tc_fence_after();
-                    const uint32_t a = smem_u32(A + (size_t)r.s * kABytes), b = smem_u32(B + (size_t)r.s * kPairB);
                     if (elect_one()) {
-#pragma unroll
-                        for (int j = 0; j < kKB / 32; j++)
-                            mma_i8<2>(tmem + (uint32_t)(buf * kPairTokens), smem_desc(a + 32 * j), smem_desc(b + 32 * j),
-                                      idesc, kb > 0 || j > 0);
-                        mma_commit<2>(&empty[r.s]);
+                        mma_stage<2>(acc, a0 + r.s * (kABytes >> 4), b0 + r.s * (kPairB >> 4), idesc, kb > 0);
+                        mma_commit<2>(empties + 8 * r.s);
                     }
                     __syncwarp();
                 }
-                if (elect_one()) mma_commit<2>(&acc_full[buf]);
+                if (elect_one()) mma_commit<2>(accs + 8 * buf);
                 __syncwarp();
             }
             // the MMAs issued last have read their operands before the CTA exits
