@@ -48,7 +48,8 @@ struct GemmI8 {
     int64_t kbt;            // 128-wide columns of K
     int64_t row_tiles, token_tiles;
     int64_t whole;          // pair kernel: tiles taken whole; each later one in PARTS
-    int parts;
+    int parts, stages;
+    uint32_t b_bytes;       // of a stage's tokens in one CTA
     int* err;
 };
 
@@ -222,15 +223,16 @@ __device__ __forceinline__ bool wait_spin(uint32_t bar, uint32_t parity, int* er
     if (i == kWaitLimit) atomicExch(err, CLQ_ERR_TIMEOUT);
     return __all_sync(0xffffffffu, ok);
 }
-// A role's place in a ring of N stages: the stage and the parity of its round.
+// A role's place in a ring of n stages: the stage and the parity of its round.
 // Stepped rather than divided out of a count: the loops' rate is that of one
 // warp's instructions (a division a stage cost 0.1 us of 0.28).
-template <int N>
 struct Ring {
+    int n;
     int s = 0;
     uint32_t round = 0;
+    __device__ __forceinline__ explicit Ring(int stages) : n(stages) {}
     __device__ __forceinline__ void next() {
-        if (++s == N) {
+        if (++s == n) {
             s = 0;
             round++;
         }
@@ -404,12 +406,12 @@ __global__ void __launch_bounds__(kThreads) int8_tile_kernel(const __grid_consta
     const uint32_t fulls = smem_u32(full), empties = smem_u32(empty);
     if (warp == 4) {
         const uint32_t a0 = smem_u32(A), b0 = smem_u32(B);
-        Ring<NS> r;
+        Ring r(NS);
         int it = 0;
         bool ready = false;
         for (; it < nk; it++, r.next()) {
             if (r.round && !wait_spin(empties + 8 * r.s, r.parity() ^ 1u, G.err, ready)) break;
-            const Ring<NS> next = r.after();
+            const Ring next = r.after();
             ready = next.round && peek(empties + 8 * next.s, next.parity() ^ 1u);
             if (elect_one()) {
                 arrive_tx(fulls + 8 * r.s, kABytes + kBBytes);
@@ -423,11 +425,11 @@ __global__ void __launch_bounds__(kThreads) int8_tile_kernel(const __grid_consta
     } else if (warp == 5) {
         const uint32_t a0 = desc_low(smem_u32(A)), b0 = desc_low(smem_u32(B));
         constexpr uint32_t idesc = instr_desc_i8(kRows, TN);
-        Ring<NS> r;
+        Ring r(NS);
         bool ready = false;
         for (int it = 0; it < nk; it++, r.next()) {
             if (!wait_spin(fulls + 8 * r.s, r.parity(), G.err, ready)) break;
-            const Ring<NS> next = r.after();
+            const Ring next = r.after();
             ready = peek(fulls + 8 * next.s, next.parity());
             tc_fence_after();
             if (elect_one()) {
@@ -510,9 +512,11 @@ __global__ void __launch_bounds__(kThreads) int8_tile_kernel(const __grid_consta
 
 // ---- pair kernel --------------------------------------------------------------
 
-constexpr int kPairTokens = 256, kPairStages = 6, kGroup = 8;
+constexpr int kPairTokens = 256, kGroup = 8;
 constexpr uint32_t kPairB = kPairTokens / 2 * kKB;  // each CTA stages half of the tokens
-constexpr size_t kPairSmem = 1024 + (size_t)kPairStages * (kABytes + kPairB) + (2 * kPairStages + 4) * 8 + 16;
+constexpr uint32_t kPairRing = 6 * (kABytes + kPairB);  // six stages, or up to ten of fewer tokens
+constexpr int kPairMaxStages = 10;
+constexpr size_t kPairSmem = 1024 + kPairRing + (2 * kPairMaxStages + 4) * 8 + 16;
 static_assert(kPairSmem <= kSmemPerSm, "shared memory of one SM");
 
 // What a pair of SMs does at one time: rows [256 RT, ..) for TOKENS tokens from T0 on.
@@ -541,12 +545,12 @@ __device__ __forceinline__ PairUnit pair_unit(const GemmI8& G, int64_t unit) {
 template <typename OT>
 __global__ void __launch_bounds__(kThreads, 1) int8_pair_kernel(const __grid_constant__ GemmI8 G) {
     extern __shared__ __align__(1024) uint8_t smem_raw[];
-    constexpr int NS = kPairStages;
+    const int NS = G.stages;
     uint8_t* A = align1024(smem_raw);
     uint8_t* B = A + (size_t)NS * kABytes;
-    uint64_t* full = reinterpret_cast<uint64_t*>(B + (size_t)NS * kPairB);  // used in the leader
-    uint64_t* empty = full + NS;                                            // in both
-    uint64_t* acc_full = empty + NS;                                        // [2], in both
+    uint64_t* full = reinterpret_cast<uint64_t*>(A + kPairRing);            // used in the leader
+    uint64_t* empty = full + kPairMaxStages;                                // in both
+    uint64_t* acc_full = empty + kPairMaxStages;                            // [2], in both
     uint64_t* acc_empty = acc_full + 2;                                     // [2], in the leader
     uint32_t* slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
 
@@ -559,7 +563,8 @@ __global__ void __launch_bounds__(kThreads, 1) int8_pair_kernel(const __grid_con
     const int nk = (int)G.kbt;
 
     if (warp == 5) {
-        if (lane < 2 * NS + 4) mbar_init(full + lane, lane < 2 * NS + 2 ? 1 : 8);  // acc_empty: both CTAs' epilogue warps
+        if (lane < 2 * kPairMaxStages + 4)  // acc_empty: both CTAs' epilogue warps
+            mbar_init(full + lane, lane < 2 * kPairMaxStages + 2 ? 1 : 8);
         mbar_init_fence();
     } else if (warp == 4) {
         if (lane < 3) prefetch_map(lane == 0 ? &G.wmap : lane == 1 ? &G.xmap : &G.xmap_part);
@@ -578,7 +583,7 @@ __global__ void __launch_bounds__(kThreads, 1) int8_pair_kernel(const __grid_con
     const uint32_t fulls = smem_u32(full), empties = smem_u32(empty);
     if (warp == 4) {
         const uint32_t a0 = smem_u32(A), b0 = smem_u32(B), fulls_leader = map_rank(fulls, 0);
-        Ring<NS> r;
+        Ring r(NS);
         bool ok = true, ready = false;
         for (int64_t tile = first; tile < tiles && ok; tile += step) {
             const PairUnit u = pair_unit(G, tile);
@@ -588,12 +593,12 @@ __global__ void __launch_bounds__(kThreads, 1) int8_pair_kernel(const __grid_con
             const uint32_t tx = 2u * (kABytes + (uint32_t)u.tokens / 2 * kKB);
             for (int kb = 0; kb < nk; kb++, r.next()) {
                 if (r.round && !(ok = wait_spin(empties + 8 * r.s, r.parity() ^ 1u, G.err, ready))) break;
-                const Ring<NS> next = r.after();
+                const Ring next = r.after();
                 ready = next.round && peek(empties + 8 * next.s, next.parity() ^ 1u);
                 if (elect_one()) {
                     if (leader) arrive_tx(fulls + 8 * r.s, tx);
                     copy_box<2>(a0 + r.s * kABytes, &G.wmap, kb * kKB, y_w, fulls_leader + 8 * r.s);
-                    copy_box<2>(b0 + r.s * kPairB, xmap, kb * kKB, y_x, fulls_leader + 8 * r.s);
+                    copy_box<2>(b0 + r.s * G.b_bytes, xmap, kb * kKB, y_x, fulls_leader + 8 * r.s);
                 }
                 __syncwarp();
             }
@@ -607,7 +612,7 @@ __global__ void __launch_bounds__(kThreads, 1) int8_pair_kernel(const __grid_con
     } else if (warp == 5) {
         if (leader) {
             const uint32_t a0 = desc_low(smem_u32(A)), b0 = desc_low(smem_u32(B)), accs = smem_u32(acc_full);
-            Ring<NS> r;
+            Ring r(NS);
             int64_t nt = 0;
             bool ok = true, ready = false;
             for (int64_t tile = first; tile < tiles && ok; tile += step, nt++) {
@@ -619,11 +624,11 @@ __global__ void __launch_bounds__(kThreads, 1) int8_pair_kernel(const __grid_con
                 tc_fence_after();
                 for (int kb = 0; kb < nk; kb++, r.next()) {
                     if (!(ok = wait_spin(fulls + 8 * r.s, r.parity(), G.err, ready))) break;
-                    const Ring<NS> next = r.after();
+                    const Ring next = r.after();
                     ready = peek(fulls + 8 * next.s, next.parity());
                     tc_fence_after();
                     if (elect_one()) {
-                        mma_stage<2>(acc, a0 + r.s * (kABytes >> 4), b0 + r.s * (kPairB >> 4), idesc, kb > 0);
+                        mma_stage<2>(acc, a0 + r.s * (kABytes >> 4), b0 + r.s * (G.b_bytes >> 4), idesc, kb > 0);
                         mma_commit<2>(empties + 8 * r.s);
                     }
                     __syncwarp();
@@ -706,6 +711,9 @@ cudaError_t launch_pair(GemmI8& g, cudaStream_t s) {
     if (!make_maps(&g, kRows, kPairTokens / 2) ||
         !encode_swizzled_rows(&g.xmap_part, g.p.x, g.p.m, g.p.k, g.p.ldx, kPairTokens / 2 / g.parts))
         return cudaErrorNotSupported;
+    // where every unit is a part, the ring holds more stages of fewer tokens
+    g.b_bytes = kPairB / (g.whole ? 1u : (uint32_t)g.parts);
+    g.stages = std::min<int>(kPairMaxStages, (int)(kPairRing / (kABytes + g.b_bytes)));
     static std::atomic<uint64_t> allowed{0};
     const cudaError_t e = allow_smem(int8_pair_kernel<OT>, kPairSmem, allowed);
     if (e != cudaSuccess) return e;
