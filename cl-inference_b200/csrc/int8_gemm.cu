@@ -353,14 +353,20 @@ __device__ __forceinline__ void join_parts(const Int8Product& P, uint32_t at, in
 
 // ---- tile kernel --------------------------------------------------------------
 
-// 32 tokens: half of an SM's shared memory, so that the next launch's CTAs can
-// start beside the last ones (24 x 4096 x 4096: 7.4 us, with ten stages 7.7).
-constexpr int tile_stages(int tn) { return tn == 256 ? 4 : tn == 128 ? 6 : tn == 64 ? 8 : 5; }
-constexpr size_t tile_smem(int tn) {
-    return 1024 + (size_t)tile_stages(tn) * (kABytes + (size_t)tn * kKB) + (2 * tile_stages(tn) + 2) * 8 + (size_t)tn * 4;
+// Stages of a CTA that has an SM to itself (for 32 tokens fewer than fit: eight cover
+// memory's latency), or shares it with one other.
+constexpr int tile_stages(int tn, int per_sm) {
+    return per_sm == 2 ? (tn == 64 ? 4 : 5) : tn == 256 ? 4 : tn == 128 ? 7 : tn == 64 ? 9 : 8;
 }
-static_assert(tile_smem(256) <= kSmemPerSm && tile_smem(128) <= kSmemPerSm && tile_smem(64) <= kSmemPerSm &&
-              tile_smem(32) <= kSmemPerSm, "shared memory of one SM");
+constexpr size_t tile_smem(int tn, int stages) {
+    return 1024 + (size_t)stages * (kABytes + (size_t)tn * kKB) + (2 * stages + 2) * 8 + (size_t)tn * 4;
+}
+constexpr bool tile_fits(int tn, int per_sm) {  // with the 1 KB that the system takes of each CTA's share
+    return tile_smem(tn, tile_stages(tn, per_sm)) <= (kSmemPerSm + 1024) / per_sm - 1024 &&
+           (size_t)tn * kRows * 4 <= (size_t)tile_stages(tn, per_sm) * (kABytes + (size_t)tn * kKB);  // the sums, over them
+}
+static_assert(tile_fits(256, 1) && tile_fits(128, 1) && tile_fits(64, 1) && tile_fits(32, 1) && tile_fits(64, 2) &&
+              tile_fits(32, 2), "shared memory");
 
 // CTA (blockIdx.x = row tile x SPLITS + part, blockIdx.y = token tile); the
 // SPLITS parts of a tile form a cluster.  Each part leaves its sums in its own
@@ -369,9 +375,8 @@ static_assert(tile_smem(256) <= kSmemPerSm && tile_smem(128) <= kSmemPerSm && ti
 template <typename OT, int TN>
 __global__ void __launch_bounds__(kThreads) int8_tile_kernel(const __grid_constant__ GemmI8 G, int splits) {
     extern __shared__ __align__(1024) uint8_t smem_raw[];
-    constexpr int NS = tile_stages(TN);
+    const int NS = G.stages;
     constexpr uint32_t kBBytes = TN * kKB;
-    static_assert((size_t)TN * kRows * 4 <= (size_t)NS * (kABytes + kBBytes), "the sums fit over the stages");
     uint8_t* A = align1024(smem_raw);
     uint8_t* B = A + (size_t)NS * kABytes;
     int* sums = reinterpret_cast<int*>(A);
@@ -421,7 +426,8 @@ __global__ void __launch_bounds__(kThreads) int8_tile_kernel(const __grid_consta
             __syncwarp();
         }
         // what is in flight lands before the CTA exits
-        for (int i = it < NS ? 0 : it - NS; i < it; i++) mbar_drain(&full[i % NS], (i / NS) & 1);
+        for (int i = 0; i < NS; i++, r.next())
+            if (r.round) mbar_drain(&full[r.s], r.parity() ^ 1u);
     } else if (warp == 5) {
         const uint32_t a0 = desc_low(smem_u32(A)), b0 = desc_low(smem_u32(B));
         constexpr uint32_t idesc = instr_desc_i8(kRows, TN);
@@ -683,12 +689,13 @@ bool make_maps(GemmI8* g, int w_box, int x_box) {
 }
 
 template <typename OT, int TN>
-cudaError_t launch_tile(GemmI8& g, int splits, cudaStream_t s) {
+cudaError_t launch_tile(GemmI8& g, int splits, int per_sm, cudaStream_t s) {
     const int64_t rt = (g.p.n + kRows - 1) / kRows, tt = (g.p.m + TN - 1) / TN;
     if (rt * splits > INT32_MAX || tt > 65535 || !make_maps(&g, kRows, TN)) return cudaErrorNotSupported;
-    const size_t smem = tile_smem(TN);
+    g.stages = tile_stages(TN, per_sm);
+    const size_t smem = tile_smem(TN, g.stages);
     static std::atomic<uint64_t> allowed{0};
-    const cudaError_t e = allow_smem(int8_tile_kernel<OT, TN>, smem, allowed);
+    const cudaError_t e = allow_smem(int8_tile_kernel<OT, TN>, tile_smem(TN, tile_stages(TN, 1)), allowed);
     if (e != cudaSuccess) return e;
     return launch_cluster(int8_tile_kernel<OT, TN>, dim3((unsigned)(rt * splits), (unsigned)tt), kThreads, smem, splits, s, g,
                           splits);
@@ -731,7 +738,7 @@ int resident_clusters(int splits) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(splits * sm_count()));
     cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = tile_smem(256);
+    cfg.dynamicSmemBytes = tile_smem(256, tile_stages(256, 1));
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = (unsigned)splits;
@@ -754,19 +761,19 @@ int resident_clusters(int splits) {
 // with c a 128-byte column's time and e a tile's start and end, fitted to every
 // variant at 1024 to 14336 rows and K = 2051 to 14336.  What it decides, at K =
 // 4096 (us; the tile kernel as tokens / parts of K):
-//   24 tokens, 4096 rows    32/4  7.4   32/1 11.6   pair 12.9
-//   128 tokens, 4096 rows   64/2  9.8   128/1 13.4  pair 13.6
-//   256 tokens, 6144 rows   128/1 14.2  pair 15.1   256/2 16.4
-//   256 tokens, 14336 rows  pair 19.4   256/1 22.2  128/1 28.5
-//   512 tokens, 4096 rows, K = 14336:  256/2 31.9  128/1 37.1  pair 37.7
+//   24 tokens, 4096 rows    32/4  7.2   32/1  9.1   pair 10.9
+//   128 tokens, 4096 rows   64/2  9.0   64/1  9.5   pair 11.5
+//   256 tokens, 6144 rows   128/1 11.9  pair 13.2   256/2 16.1
+//   256 tokens, 14336 rows  pair 19.6   256/1 21.4  128/1 24.9
+//   512 tokens, 4096 rows, K = 14336:  128/1 29.4  pair 30.4  256/2 31.0
 struct Choice {
-    int tn, splits;  // tn 0: the pair kernel
+    int tn, splits, per_sm;  // tn 0: the pair kernel
 };
 Choice choose(const Int8Product& p, int64_t kbt) {
     static const struct {
         int tn;
-        double c, e1, es;  // es: with K split
-    } kTiles[] = {{32, 0.255, 1.2, 2.6}, {64, 0.255, 1.8, 3.4}, {128, 0.27, 2.8, 5.0}, {256, 0.34, 4.4, 8.4}};
+        double c, e1, es, c2;  // es: with K split; c2: two to an SM
+    } kTiles[] = {{32, 0.185, 1.15, 2.4, 0.45}, {64, 0.19, 1.5, 3.4, 0.55}, {128, 0.218, 2.3, 5.0, 0.}, {256, 0.364, 3.8, 7.9, 0.}};
     static const int kSplits[] = {1, 2, 3, 4, 6, 8};
     const auto rounds = [](int64_t tiles, int64_t at_once) { return (double)((tiles + at_once - 1) / at_once); };
     const double traffic = (double)(p.n + p.m) * (double)p.k / 6.2e6;
@@ -774,9 +781,9 @@ Choice choose(const Int8Product& p, int64_t kbt) {
     const int64_t pairs = sm_count() / 2;
     const int parts = parts_of(units % pairs, pairs);
     // the pair kernel's tiles overlap: only the last one's end, shorter in parts, is waited for
-    Choice best = {0, 1};
-    double least = (double)kbt * (0.35 * (double)(units / pairs) + (units % pairs ? parts > 1 ? 0.28 : 0.335 : 0.));
-    least = std::max(least, traffic) + (units % pairs == 0 || parts == 1 ? 4.5 : parts == 2 ? 4.0 : parts == 4 ? 2.8 : 2.5);
+    Choice best = {0, 1, 1};
+    double least = (double)kbt * (0.35 * (double)(units / pairs) + (units % pairs ? parts > 1 ? 0.225 : 0.322 : 0.));
+    least = std::max(least, traffic) + (units % pairs == 0 || parts == 1 ? 5.0 : parts == 2 ? 3.85 : parts == 4 ? 2.5 : 2.3);
     for (const auto& t : kTiles) {
         const int64_t tiles = ((p.n + kRows - 1) / kRows) * ((p.m + t.tn - 1) / t.tn);
         if ((p.m + t.tn - 1) / t.tn > 65535) continue;
@@ -784,9 +791,19 @@ Choice choose(const Int8Product& p, int64_t kbt) {
             if (splits > 1 && 2 * splits > kbt) break;
             const double r = rounds(tiles, resident_clusters(splits));
             const double cost = std::max(r * (double)((kbt + splits - 1) / splits) * t.c, traffic) + r * (splits > 1 ? t.es : t.e1);
+            if (cost <= least) {  // of equals, more parts: their copies are under way sooner
+                least = cost;
+                best = {t.tn, splits, 1};
+            }
+        }
+        // more tiles than SMs: two to an SM, each at about half of its rate (32 tokens, 28672 rows
+        // of 4096: 22.5 us, one to an SM 25.5; of 8192: 40.7 and 44.4)
+        if (t.c2 > 0 && tiles > sm_count()) {
+            const double r = rounds(tiles, 2 * sm_count());
+            const double cost = std::max(r * (double)kbt * t.c2, traffic) + r * t.e1;
             if (cost < least) {
                 least = cost;
-                best = {t.tn, splits};
+                best = {t.tn, 1, 2};
             }
         }
     }
@@ -797,10 +814,10 @@ template <typename OT>
 cudaError_t launch_type(GemmI8& g, cudaStream_t s) {
     const Choice c = choose(g.p, g.kbt);
     switch (c.tn) {
-    case 32: return launch_tile<OT, 32>(g, c.splits, s);
-    case 64: return launch_tile<OT, 64>(g, c.splits, s);
-    case 128: return launch_tile<OT, 128>(g, c.splits, s);
-    case 256: return launch_tile<OT, 256>(g, c.splits, s);
+    case 32: return launch_tile<OT, 32>(g, c.splits, c.per_sm, s);
+    case 64: return launch_tile<OT, 64>(g, c.splits, c.per_sm, s);
+    case 128: return launch_tile<OT, 128>(g, c.splits, c.per_sm, s);
+    case 256: return launch_tile<OT, 256>(g, c.splits, c.per_sm, s);
     default: return launch_pair<OT>(g, s);
     }
 }

@@ -164,6 +164,10 @@ cudaError_t launch_gv_type(const Int8Product& p, cudaStream_t s) {
 
 cudaError_t launch_int8_gemv(const Int8Product& p, cudaStream_t s) {
     if (p.m > 16 || !int8_aligned(p)) return cudaErrorNotSupported;
+    // the second half of the tokens' loads costs a fifth of the rate, the tile kernel 2 us more to
+    // start: sixteen tokens at 28672 x 8192 46.6 us here and 40.7 there, at 14336 x 4096 13.8
+    // and 12.9, at 4096 x 4096 5.6 and 7.0
+    if (p.m > 8 && p.n * p.k > 40 * 1000 * 1000) return cudaErrorNotSupported;
     switch (p.otype) {
     case CLQ_X_F32: return launch_gv_type<float>(p, s);
     case CLQ_X_BF16: return launch_gv_type<__nv_bfloat16>(p, s);

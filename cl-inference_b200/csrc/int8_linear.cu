@@ -94,7 +94,8 @@ bool int8_aligned(const Int8Product& p) {
 
 cudaError_t launch_linear_int8(const Int8Product& p, cudaStream_t s) {
     if (p.k < 1 || !int8_aligned(p)) return launch_linear_int8_generic(p, s);
-    cudaError_t e = p.m <= 16 ? launch_int8_gemv(p, s) : launch_int8_gemm(p, s);
+    cudaError_t e = launch_int8_gemv(p, s);
+    if (e == cudaErrorNotSupported) e = launch_int8_gemm(p, s);
     return e == cudaErrorNotSupported ? launch_linear_int8_generic(p, s) : e;
 }
 
