@@ -53,7 +53,7 @@ def _plain(t, dtype, dims):
     """Whether T is a tensor of that type and rank on the current device with
     unit last stride: what nearly every call has, told in one go."""
     return (type(t) is _t.Tensor and t.dtype is dtype and t.dim() == dims and t.is_cuda and t.get_device() == _device()
-            and t.stride(-1) == 1)
+            and t.stride(dims - 1) == 1)
 
 
 def _matrix(t, what, shape=None):
@@ -113,11 +113,11 @@ class Int8Rows:
 
     def __init__(self, codes, scales):
         torch = _t or _torch()
-        if not _plain(codes, torch.int8, 2):
+        if not (_plain(codes, torch.int8, 2) and _plain(scales, torch.float32, 1)
+                and scales.shape[0] == codes.shape[0]):
             codes = _matrix(codes, "codes")
             if codes.dtype != torch.int8:
                 raise ValueError(f"codes: int8, not {codes.dtype}")
-        if not _plain(scales, torch.float32, 1) or scales.shape[0] != codes.shape[0]:
             scales = _vector(scales, codes.shape[0], "scales")
         self.codes, self.scales = codes, scales
 
@@ -141,18 +141,24 @@ class Int8Rows:
         if stream is not None:
             return _on(stream, (codes, scales, out), lambda: self.dequantize(dtype, out))
         m, k = codes.shape
-        device = _here(codes, "codes")
+        device = _device()
+        if codes.get_device() != device:
+            _here(codes, "codes")
         if dtype is None:
             dtype = torch.float32 if out is None else out.dtype
-        code = _type_code(dtype, "dtype")
+        code = _types.get(dtype)
+        if code is None:
+            _type_code(dtype, "dtype")
+        ldo = k
         if out is not None:
             _writable(out, "out", (m, k), dtype)
+            ldo = _ld(out, m, k)
         elif codes.is_contiguous():
             out = torch.empty_like(codes, dtype=dtype)
         else:
             out = codes.new_empty((m, k), dtype=dtype)
-        status = _lib_dequantize(codes.data_ptr(), _ld(codes, m, k), scales.data_ptr(), m, k, out.data_ptr(), code,
-                                 _ld(out, m, k), _stream(device))
+        status = _lib_dequantize(codes.data_ptr(), _ld(codes, m, k), scales.data_ptr(), m, k, out.data_ptr(), code, ldo,
+                                 _stream(device))
         if status:
             _lib.check(status)
         return out
@@ -260,26 +266,33 @@ def linear_int8(x, w, out=None, dtype=None, residual=None, stream=None):
     n, wk = wc.shape
     if wk != k:
         raise ValueError(f"rows of {k} codes against a weight of {tuple(wc.shape)}")
-    device = _here(xc, "x")
-    if wc.get_device() != device:
+    device = _device()
+    if xc.get_device() != device or wc.get_device() != device:
+        _here(xc, "x")
         _here(wc, "w")
     if dtype is None:
         dtype = torch.float32 if out is None else out.dtype
-    code = _type_code(dtype, "dtype")
-    rptr, ldr = None, 0
+    code = _types.get(dtype)
+    if code is None:
+        _type_code(dtype, "dtype")
+    rptr, ldr, ldo = None, 0, n
     if out is not None:
         _writable(out, "out", (m, n), dtype)
+        ldo = _ld(out, m, n)
     if residual is not None:
         if out is not None:
             _apart(out, residual, "out")
-        residual = _matrix(residual, "residual", (m, n))
-        if residual.dtype != torch.float32:
-            raise ValueError(f"residual: float32, not {residual.dtype}")
+        if not _plain(residual, torch.float32, 2) or residual.shape != (m, n):
+            residual = _matrix(residual, "residual", (m, n))
+            if residual.dtype != torch.float32:
+                raise ValueError(f"residual: float32, not {residual.dtype}")
         rptr, ldr = residual.data_ptr(), _ld(residual, m, n)
     if out is None:
         out = xc.new_empty((m, n), dtype=dtype)
-    status = _lib_linear(xc.data_ptr(), _ld(xc, m, k), x.scales.data_ptr(), m, wc.data_ptr(), _ld(wc, n, k), w.scales.data_ptr(),
-                         n, k, rptr, ldr, out.data_ptr(), code, _ld(out, m, n), _stream(device))
+    single = (k + 15) // 16 * 16  # one row has no stride to speak of
+    status = _lib_linear(xc.data_ptr(), xc.stride(0) if m > 1 else single, x.scales.data_ptr(), m, wc.data_ptr(),
+                         wc.stride(0) if n > 1 else single, w.scales.data_ptr(), n, k, rptr, ldr, out.data_ptr(), code, ldo,
+                         _stream(device))
     if status:
         _lib.check(status)
     return out
