@@ -69,6 +69,9 @@ int i8_fail(int code, const char* what) { return set_error(code, "%s", what); }
 
 bool known_type(int t) { return t == CLQ_X_F32 || t == CLQ_X_BF16 || t == CLQ_X_F16; }
 
+// Whether P may hold elements of TYPE: kernels load whole ones.
+bool off_type(const void* p, int type) { return (uintptr_t)p % (type == CLQ_X_F32 ? 4 : 2) != 0; }
+
 int check_codes(const char* what, int64_t m, int64_t k, int64_t ld) {
     if (m < 0 || k < 0) return set_error(CLQ_ERR_SHAPE, "%s: negative shape (%lld %lld)", what, (long long)m, (long long)k);
     if (ld < k && m > 1)
@@ -81,6 +84,9 @@ int run_quantize(const QuantRows& q, void* stream) {
     if (q.m == 0) return CLQ_OK;
     if (q.k > 0 && (!q.x || !q.codes)) return i8_fail(CLQ_ERR_ARGUMENT, "null rows or codes");
     if (!q.scales) return i8_fail(CLQ_ERR_ARGUMENT, "null scales");
+    if (off_type(q.x, q.xtype) || off_type(q.gate, q.xtype) || off_type(q.res, q.rtype) || off_type(q.res_out, q.rtype) ||
+        off_type(q.norm_w, CLQ_X_F32) || off_type(q.scales, CLQ_X_F32))
+        return i8_fail(CLQ_ERR_ARGUMENT, "an address off its element type's alignment");
     if ((rc = sm100_device(&dev))) return rc;
     const cudaError_t e = launch_quantize_rows(q, (cudaStream_t)stream);
     return e == cudaSuccess ? CLQ_OK : set_error(CLQ_ERR_CUDA, "row quantization: %s", cudaGetErrorString(e));
@@ -180,6 +186,8 @@ int clq_dequantize_rows_device(const int8_t* codes, int64_t ldc, const float* sc
     if ((rc = clq::check_codes("values", m, k, ldo))) return rc;
     if (m == 0 || k == 0) return CLQ_OK;
     if (!codes || !scales || !out) return i8_fail(CLQ_ERR_ARGUMENT, "null codes, scales or output");
+    if (clq::off_type(scales, CLQ_X_F32) || clq::off_type(out, otype))
+        return i8_fail(CLQ_ERR_ARGUMENT, "an address off its element type's alignment");
     if ((rc = clq::sm100_device(&dev))) return rc;
     const cudaError_t e = clq::launch_dequantize_rows(codes, ldc, scales, m, k, out, otype, ldo, (cudaStream_t)stream);
     return e == cudaSuccess ? CLQ_OK : clq::set_error(CLQ_ERR_CUDA, "row dequantization: %s", cudaGetErrorString(e));
@@ -200,6 +208,9 @@ int clq_linear_int8_device(const int8_t* x, int64_t ldx, const float* x_scales, 
         return i8_fail(CLQ_ERR_SHAPE, "the residual and the output are one matrix with two layouts");
     if (m == 0 || n == 0) return CLQ_OK;
     if (!out || !x_scales || !w_scales || (k > 0 && (!x || !w))) return i8_fail(CLQ_ERR_ARGUMENT, "null operand or output");
+    if (clq::off_type(x_scales, CLQ_X_F32) || clq::off_type(w_scales, CLQ_X_F32) || clq::off_type(residual, CLQ_X_F32) ||
+        clq::off_type(out, otype))
+        return i8_fail(CLQ_ERR_ARGUMENT, "an address off its element type's alignment");
     if ((rc = clq::sm100_device(&dev))) return rc;
     clq::Int8Product p = {};
     p.x = x;

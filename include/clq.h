@@ -343,8 +343,9 @@ int clq_attend_device(const float *q, int64_t count, int n_heads, int64_t q_pos_
  * clamp(round-half-even(v / step), -127, 127), the quotient formed as a product
  * with the rounded 1 / step; an all-zero row has the scale 1, and a row with a
  * non-finite value has codes 0 and the scale NaN.  Row strides are in elements;
- * each row is contiguous.  Any alignment is taken; code rows that start on
- * 16-byte boundaries (base and stride) run on the fast kernels.  All calls are
+ * each row is contiguous.  Any address that its element type allows is taken
+ * (others are CLQ_ERR_ARGUMENT); code rows that start on 16-byte boundaries (base
+ * and stride) run on the fast kernels.  All calls are
  * asynchronous on STREAM, allocate nothing and keep nothing.
  */
 /* M rows of K elements of XTYPE (clq_xtype). */

@@ -70,6 +70,25 @@ def test_product_checks_arguments(clq):
     assert call(n=0, w=None, ws=None, ldo=0) == 0
 
 
+def test_addresses_off_their_type_are_refused(clq):
+    def norm(x=FAKE, xtype=1, w=FAKE, res=FAKE, rtype=0, out=FAKE + 256, codes=FAKE, scales=FAKE):
+        return c(clq, "clq_norm_quantize_device", x, xtype, 2, 8, 8, w, 1e-5, res, rtype, 8, out, 8, codes, 8, scales, None)
+    for bad in (dict(x=FAKE + 1), dict(w=FAKE + 2), dict(res=FAKE + 2), dict(out=FAKE + 258), dict(scales=FAKE + 2),
+                dict(x=FAKE + 2, xtype=0)):
+        assert norm(**bad) == 1, bad
+        assert "alignment" in clq._lib.last_error()
+    assert c(clq, "clq_swiglu_quantize_device", FAKE + 1, 8, FAKE, 8, 2, 2, 8, FAKE, 8, FAKE, None) == 1
+    assert c(clq, "clq_swiglu_quantize_device", FAKE, 8, FAKE + 1, 8, 2, 2, 8, FAKE, 8, FAKE, None) == 1
+    assert c(clq, "clq_dequantize_rows_device", FAKE, 8, FAKE + 2, 2, 8, FAKE, 1, 8, None) == 1
+    assert c(clq, "clq_dequantize_rows_device", FAKE, 8, FAKE, 2, 8, FAKE + 1, 1, 8, None) == 1
+
+    def product(xs=FAKE, ws=FAKE, res=None, out=FAKE, otype=1):
+        return c(clq, "clq_linear_int8_device", FAKE, 64, xs, 2, FAKE, 64, ws, 3, 64, res, 3, out, otype, 3, None)
+    for bad in (dict(xs=FAKE + 1), dict(ws=FAKE + 2), dict(res=FAKE + 2), dict(out=FAKE + 1), dict(out=FAKE + 2, otype=0)):
+        assert product(**bad) == 1, bad
+        assert "alignment" in clq._lib.last_error()
+
+
 def test_valid_calls_need_a_device(clq):
     import torch
     if torch.cuda.is_available():
