@@ -436,6 +436,8 @@ __global__ void __launch_bounds__(stream_threads(LOOSE), !LOOSE && C * 16 / (int
             const uint32_t e = o.end_element(tid - 16, k);
             if (e < (uint32_t)k) *o.place(e) = o_end;
         }
+        // a later row's bulk copy may write where an end lies now
+        if (LOOSE) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         if (tid == 0) {
             pipe::mbar_arrive_tx(&full[s], x.bytes() + (two ? o.bytes() : 0u) + (first ? wts_bytes : 0u));
             x.copy(&full[s]);
@@ -685,7 +687,7 @@ cudaError_t launch_stream(const QuantRows& q, int threads, int stages, bool wts_
 // The streaming kernel with as many CTAs to an SM (up to eight) as leave each of
 // them two buffers and, together, 1024 threads; one buffer, and the norm weight read
 // from global memory, where rows are too long for that.  cudaErrorNotSupported for
-// rows that no buffer or no 64 values a thread hold.
+// rows that no buffer holds, or more values than stream_values of each thread.
 template <typename XT, typename RT, int MODE, bool LOOSE>
 cudaError_t try_stream(const QuantRows& q, cudaStream_t s) {
     constexpr int V = 16 / (int)sizeof(XT), kStreamThreads = stream_threads(LOOSE);
