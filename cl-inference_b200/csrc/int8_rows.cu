@@ -103,22 +103,38 @@ __device__ __forceinline__ uint32_t code_bits(float v, float inv) { return __flo
 
 // ---- rows held in registers -------------------------------------------------
 
-// VALUES consecutive elements of T at P as f32: one, or VALUES * sizeof(T) a multiple
-// of 16 bytes with P on 16.
+// VALUES consecutive elements of T as they lie in memory: one, or VALUES * sizeof(T) a
+// multiple of 16 bytes with the address on 16.  Kept so until a batch of loads is
+// under way: a conversion beside each of them waits for it (2048 rows of 4097
+// bf16, an element at a time: 42 us).
 template <typename T, int VALUES>
-__device__ __forceinline__ void load_values(const T* p, float (&f)[VALUES]) {
-    if constexpr (VALUES == 1) {
-        f[0] = to_f32(*p);
-    } else {
-        constexpr int E = 16 / (int)sizeof(T);
+struct Packed {
+    static constexpr int E = 16 / (int)sizeof(T);
+    uint4 w[VALUES / E] = {};
+    __device__ __forceinline__ void load(const T* p) {
+#pragma unroll
+        for (int i = 0; i < VALUES / E; i++) w[i] = reinterpret_cast<const uint4*>(p)[i];
+    }
+    __device__ __forceinline__ void unpack(float (&f)[VALUES]) const {
 #pragma unroll
         for (int i = 0; i < VALUES / E; i++) {
-            const uint4 w = reinterpret_cast<const uint4*>(p)[i];
-            const T* e = reinterpret_cast<const T*>(&w);
+            const T* e = reinterpret_cast<const T*>(&w[i]);
 #pragma unroll
             for (int j = 0; j < E; j++) f[i * E + j] = to_f32(e[j]);
         }
     }
+};
+template <typename T>
+struct Packed<T, 1> {
+    T v = T(0.f);
+    __device__ __forceinline__ void load(const T* p) { v = *p; }
+    __device__ __forceinline__ void unpack(float (&f)[1]) const { f[0] = to_f32(v); }
+};
+template <typename T, int VALUES>
+__device__ __forceinline__ void load_values(const T* p, float (&f)[VALUES]) {
+    Packed<T, VALUES> a;
+    a.load(p);
+    a.unpack(f);
 }
 template <typename T, int VALUES>
 __device__ __forceinline__ void store_values(T* p, const float (&f)[VALUES]) {
@@ -180,11 +196,16 @@ __device__ __forceinline__ void store_codes(int8_t* p, const float (&v)[V], floa
 constexpr int kSmallRow = 128;  // threads of a CTA that takes a row per warp
 
 // CTAs an SM holds: 16 values a thread leave room for 1024 to 1280 threads, 32
-// for 1024 of f32 rows and 512 of 16-bit ones, 64 for 512.
+// for 1024 of f32 rows and 512 of 16-bit ones, 64 for 512.  Element by element, 1024
+// (more spill: 2048 x 4095 f32 norm 24.6 us, 21.4 so) and three CTAs of 384.
 template <typename XT, int V, int G, int C>
 constexpr int min_ctas() {
     constexpr int values = C * V, threads = G == 32 ? kSmallRow : G;
-    constexpr int at_once = values > (sizeof(XT) == 4 ? 32 : 16) ? 512 : values <= 16 && sizeof(XT) == 4 ? 1280 : 1024;
+    constexpr bool f32 = sizeof(XT) == 4;
+    constexpr int at_once = V == 1                   ? threads == 384 ? 1152 : 1024
+                            : values > (f32 ? 32 : 16) ? 512
+                            : values <= 16 && f32      ? 1280
+                                                       : 1024;
     return threads < at_once ? at_once / threads : 1;
 }
 
@@ -207,8 +228,10 @@ __global__ void __launch_bounds__(G == 32 ? kSmallRow : G, min_ctas<XT, step_of<
     if (row >= Q.m) return;  // whole warps, and only where no barrier follows
     const int tid = G == 32 ? threadIdx.x & 31 : threadIdx.x;
     const XT* x = static_cast<const XT*>(Q.x) + row * Q.ldx;
-    const XT* gate = MODE == kSwiglu ? static_cast<const XT*>(Q.gate) + row * Q.ldg : nullptr;
-    const RT* res = Q.res ? static_cast<const RT*>(Q.res) + row * Q.ldr : nullptr;
+    // gate (of type RT too) or residual
+    const RT* other = MODE == kSwiglu ? static_cast<const RT*>(Q.gate) + row * Q.ldg
+                      : Q.res         ? static_cast<const RT*>(Q.res) + row * Q.ldr
+                                      : nullptr;
     float v[C][V];
     float ss = 0.f, peak = 0.f;
     const int k = (int)Q.k;
@@ -217,28 +240,37 @@ __global__ void __launch_bounds__(G == 32 ? kSmallRow : G, min_ctas<XT, step_of<
     constexpr int B = C < 4 || V == 1 ? C : V * C > 32 && V == 8 ? 2 : 4;
 #pragma unroll
     for (int c0 = 0; c0 < C; c0 += B) {
-        float o[B][V];  // residual or gate
+        Packed<XT, V> xp[B];
+        Packed<RT, V> op[B];  // residual or gate
 #pragma unroll
         for (int b = 0; b < B; b++) {
             const int i = ((c0 + b) * G + tid) * V;
-#pragma unroll
-            for (int j = 0; j < V; j++) {
-                v[c0 + b][j] = 0.f;
-                o[b][j] = MODE == kSwiglu ? 0.f : -0.f;  // x + -0 is x, its sign kept
-            }
             if (i < k) {
-                load_values<XT, V>(x + i, v[c0 + b]);
-                if constexpr (MODE == kSwiglu) load_values<XT, V>(gate + i, o[b]);
-                else if (res) load_values<RT, V>(res + i, o[b]);
+                xp[b].load(x + i);
+                if constexpr (MODE == kSwiglu) op[b].load(other + i);
+            }
+        }
+        if (MODE != kSwiglu && other) {
+#pragma unroll
+            for (int b = 0; b < B; b++) {
+                const int i = ((c0 + b) * G + tid) * V;
+                if (i < k) op[b].load(other + i);
             }
         }
 #pragma unroll
         for (int b = 0; b < B; b++) {
             const int i = ((c0 + b) * G + tid) * V;
+            float o[V];
+            xp[b].unpack(v[c0 + b]);
+            op[b].unpack(o);
+            if (MODE != kSwiglu && !other) {
+#pragma unroll
+                for (int j = 0; j < V; j++) o[j] = -0.f;  // x + -0 is x, its sign kept
+            }
             if (MODE != kSwiglu && res_out && i < k) {
                 float h[V];
 #pragma unroll
-                for (int j = 0; j < V; j++) h[j] = __fadd_rn(v[c0 + b][j], o[b][j]);
+                for (int j = 0; j < V; j++) h[j] = __fadd_rn(v[c0 + b][j], o[j]);
                 store_values<RT, V>(res_out + i, h);
             }
             float w[V];
@@ -249,7 +281,7 @@ __global__ void __launch_bounds__(G == 32 ? kSmallRow : G, min_ctas<XT, step_of<
             }
 #pragma unroll
             for (int j = 0; j < V; j++) {
-                v[c0 + b][j] = value_of<MODE>(v[c0 + b][j], o[b][j], w[j], ss);
+                v[c0 + b][j] = value_of<MODE>(v[c0 + b][j], o[j], w[j], ss);
                 peak = peak_of(peak, v[c0 + b][j]);
             }
         }
@@ -484,8 +516,10 @@ __global__ void __launch_bounds__(stream_threads(LOOSE), !LOOSE && C * 16 / (int
                 x.load(i, k, v[c]);
                 if (two) o.load(i, k, ov);
                 if constexpr (MODE == kNorm) {
-                    if (wts_held || (!LOOSE && reinterpret_cast<uintptr_t>(Q.norm_w) % 16 == 0)) {
-                        load_values<float, V>((wts_held ? wts : Q.norm_w) + i, w);
+                    if (wts_held) {
+                        load_values<float, V>(wts + i, w);
+                    } else if (reinterpret_cast<uintptr_t>(Q.norm_w) % 16 == 0 && i + V <= k) {
+                        load_values<float, V>(Q.norm_w + i, w);
                     } else {
 #pragma unroll
                         for (int j = 0; j < V; j++) w[j] = i + j < k ? Q.norm_w[i + j] : 0.f;
@@ -740,12 +774,34 @@ cudaError_t launch_rows(const QuantRows& q, cudaStream_t s) {
     return launch_long<XT, RT, MODE>(q, s);
 }
 
-// Streams what is off the 16-byte grid, whose words only shared memory puts back
-// together (rows of at most 512 take a warp, an element at a time); and, of at
-// least four rows an SM, those whose arithmetic counts beside the traffic: 16-bit rows
-// (2048 x 14336 with an f32 residual and norm 60 us, a CTA per row 77; SwiGLU 35
+// Rows off the 16-byte grid, element by element: a warp a row up to 512 elements, then a
+// CTA; few rows over as many threads as help (one of 4097 f32 with norm and residual 2.8
+// us, streamed 4.1).  cudaErrorNotSupported for those that streaming serves better, whose
+// words shared memory puts back together: more than 8192 elements (2048 x 14337
+// SwiGLU bf16 50 us, so 68), and 16-bit rows alone, where an element is a
+// small part of a request (2048 x 7001 bf16 19.9 us, so 23.2; f32 23.0 and 21.9, with
+// norm and residual 65 and 39, SwiGLU 27.7 and 25.7).
+template <typename XT, typename RT, int MODE>
+cudaError_t launch_loose(const QuantRows& q, cudaStream_t s) {
+    if (q.k <= 512) return launch_held<XT, RT, MODE, true, 32, 16>(q, s);
+    if (q.m <= sm_count()) {
+        if (q.k <= 1024) return launch_held<XT, RT, MODE, true, 256, 4>(q, s);
+        if (q.k <= 4096) return launch_held<XT, RT, MODE, true, 1024, 4>(q, s);
+        if (q.k <= 8192) return launch_held<XT, RT, MODE, true, 512, 16>(q, s);
+        if (q.k <= 16384) return launch_held<XT, RT, MODE, true, 1024, 16>(q, s);
+        return cudaErrorNotSupported;
+    }
+    if (q.k <= 2048) return launch_held<XT, RT, MODE, true, 128, 16>(q, s);
+    if (q.k <= 4096) return launch_held<XT, RT, MODE, true, 256, 16>(q, s);
+    if (q.k > 8192 || (sizeof(XT) == 2 && MODE != kSwiglu && !q.res)) return cudaErrorNotSupported;
+    return q.k <= 6144 ? launch_held<XT, RT, MODE, true, 384, 16>(q, s) : launch_held<XT, RT, MODE, true, 512, 16>(q, s);
+}
+
+// Streams long rows off the 16-byte grid (launch_loose); and, of at least four rows
+// an SM, those whose arithmetic counts beside the traffic: 16-bit rows
+// (2048 x 14336 with an f32 residual and norm 59 us, a CTA per row 77; SwiGLU 35
 // and 41) and SwiGLU of long f32 ones (45 and 49).  f32 rows otherwise keep a CTA per
-// row (the norm 61 us, streamed 70).
+// row (the norm 60 us, streamed 70).
 template <typename XT, typename RT, int MODE>
 cudaError_t launch_mode(const QuantRows& q, cudaStream_t s) {
     const uint64_t bits = (uint64_t)(uintptr_t)q.x | (uint64_t)q.ldx * sizeof(XT) | (uint64_t)(uintptr_t)q.gate |
@@ -753,8 +809,8 @@ cudaError_t launch_mode(const QuantRows& q, cudaStream_t s) {
                           (uint64_t)q.ldr * sizeof(RT) | (uint64_t)(uintptr_t)q.res_out | (uint64_t)q.ldro * sizeof(RT) |
                           (uint64_t)(uintptr_t)q.codes * 2 | (uint64_t)q.ldc * 2 | (uint64_t)q.k * sizeof(XT);
     if (bits & 15) {
-        if (q.k <= 512) return launch_held<XT, RT, MODE, true, 32, 16>(q, s);
-        const cudaError_t e = try_stream<XT, RT, MODE, true>(q, s);
+        cudaError_t e = launch_loose<XT, RT, MODE>(q, s);
+        if (e == cudaErrorNotSupported) e = try_stream<XT, RT, MODE, true>(q, s);
         return e != cudaErrorNotSupported ? e : launch_long<XT, RT, MODE>(q, s);
     }
     const bool dense = sizeof(XT) == 2 || (MODE == kSwiglu && q.k > 8192);

@@ -154,6 +154,20 @@ def test_rows_off_the_grid_at_length(cuda, clq, m, k, xtype, rtype):
     assert status(clq) == 0
 
 
+@pytest.mark.parametrize("m,k", [(3, 1023), (3, 1025), (148, 4095), (3, 4099), (3, 8191), (3, 8193), (4, 16383), (4, 16385),
+                                 (149, 4095), (300, 777), (300, 2047), (300, 2049), (300, 4097), (300, 6143), (300, 6145),
+                                 (300, 8191), (300, 8193), (200, 14337)])
+@pytest.mark.parametrize("xtype,rtype", [("float32", "float32"), ("bfloat16", "bfloat16"), ("float16", "float32")])
+def test_rows_off_the_grid_at_the_edges_of_each_split(cuda, clq, m, k, xtype, rtype):
+    test_rows_off_the_grid_at_length(cuda, clq, m, k, xtype, rtype)
+    # a norm without a residual
+    torch = cuda
+    x = rand(torch, m, k, seed=4).to(getattr(torch, xtype))
+    g = rand(torch, k, seed=5, scale=0.3) + 1
+    h = x.double()
+    check_rows(torch, clq.norm_quantize(x, g, 1e-5), h * g.double(), 1 / torch.sqrt((h * h).mean(1) + 1e-5))
+
+
 @pytest.mark.parametrize("m", [600, 1000])
 @pytest.mark.parametrize("k", [1024, 4096, 14336])
 def test_many_rows(cuda, clq, m, k):
