@@ -210,9 +210,9 @@ struct Int8Product {
     int64_t ldo;
 };
 cudaError_t launch_linear_int8(const Int8Product& p, cudaStream_t stream);
-// The kernels behind it.  Rows on 16-byte boundaries (int8_aligned) for all but
-// the generic one; cudaErrorNotSupported, before anything is launched, for a
-// request that one does not take.
+// The kernels behind it: the first for up to 16 tokens, the second for rows on 16-byte
+// boundaries (int8_aligned); cudaErrorNotSupported, before anything is launched, for
+// a request that one does not take.
 bool int8_aligned(const Int8Product& p);
 cudaError_t launch_int8_gemv(const Int8Product& p, cudaStream_t stream);
 cudaError_t launch_int8_gemm(const Int8Product& p, cudaStream_t stream);

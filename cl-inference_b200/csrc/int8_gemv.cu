@@ -14,6 +14,7 @@
 
 #include "../../include/clq.h"
 #include "clq_internal.h"
+#include "int8_mma.cuh"
 #include "int8_out.cuh"
 #include "launch.cuh"
 #include "pipeline.cuh"
@@ -44,14 +45,6 @@ __device__ __forceinline__ uint4 load_token(const int8_t* p, bool in) {
     return v;
 }
 
-__device__ __forceinline__ void mma_s8(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                       uint32_t b1) {
-    asm volatile(
-        "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-
 // Bytes [k0, k0 + 16) of a row of K codes, zeros past its end.
 __device__ __forceinline__ uint4 load_tail(const int8_t* row, int64_t k0, int64_t k) {
     if (k0 + 16 <= k) return *reinterpret_cast<const uint4*>(row + k0);
@@ -61,8 +54,10 @@ __device__ __forceinline__ uint4 load_tail(const int8_t* row, int64_t k0, int64_
 }
 
 // HI: tokens 8..15 are present.  R: groups of eight weight rows to a CTA.  W:
-// warps.  U: 64-byte columns a warp has in flight.
-template <typename OT, int R, bool HI, int W, int U>
+// warps.  U: 64-byte columns a warp has in flight.  LOOSE: rows of any address
+// and stride, at twice the loads and their shifts (one token, 4096 x 4096: 9.5 us beside
+// 4.9; 14336 x 4096: 30.3 and 11.9).
+template <typename OT, int R, bool HI, int W, int U, bool LOOSE>
 __global__ void __launch_bounds__(W * 32, 16 / W) int8_gemv_kernel(const Int8Product P) {
     __shared__ int part[W][R][HI ? 4 : 2][32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, q = lane & 3;
@@ -71,7 +66,7 @@ __global__ void __launch_bounds__(W * 32, 16 / W) int8_gemv_kernel(const Int8Pro
     // into L2, where anything that kernel still writes to them stays visible (a
     // layer of 4096 / 14336 at one token 36.7 -> 35.6 us, of 2048 / 8192 17.4 -> 16.1;
     // whole rows ahead push out the stream's own lines: 41.0).
-    if (threadIdx.x < 8 * R && n0 + threadIdx.x < P.n) {
+    if (!LOOSE && threadIdx.x < 8 * R && n0 + threadIdx.x < P.n) {
         const uint32_t bytes = (uint32_t)(P.k < W * U * 64 ? P.k & ~(int64_t)15 : W * U * 64);
         if (bytes) pipe::prefetch_l2(P.w + (n0 + threadIdx.x) * P.ldw, bytes);
     }
@@ -96,27 +91,72 @@ __global__ void __launch_bounds__(W * 32, 16 / W) int8_gemv_kernel(const Int8Pro
             mma_s8(acc[r], a.z, b.z, a.w, b.w, w[r].z, w[r].w);
         }
     };
-    const int64_t whole = P.k / 64;
-    int64_t c = warp;
-    for (; c + (U - 1) * W < whole; c += U * W) {
-        uint4 w[U][R], a[U], b[U];
+    if constexpr (LOOSE) {
+        const auto some = [&](int64_t c) {  // one column, wherever it lies
+            const int64_t k0 = c * 64 + 16 * q;
+            uint4 w[R];
+            Codes16 t;
 #pragma unroll
-        for (int u = 0; u < U; u++) {
-            const int64_t k0 = (c + u * W) * 64 + 16 * q;
-#pragma unroll
-            for (int r = 0; r < R; r++) w[u][r] = load_stream(wr[r] + k0);
-            a[u] = load_token(xlo + k0, lo_in);
-            b[u] = HI ? load_token(xhi + k0, hi_in) : zero;
+            for (int r = 0; r < R; r++) {
+                t.load(wr[r], k0, P.k);
+                w[r] = t.codes();
+            }
+            Codes16 lo, hi;
+            lo.load(xlo, k0, lo_in ? P.k : 0);
+            hi.load(xhi, k0, hi_in ? P.k : 0);
+            column(w, lo.codes(), hi.codes());
+        };
+        // the first column and the last ones have no codes on one side
+        const int64_t whole = (P.k - 16) / 64;
+        int64_t c = warp;
+        if (c == 0 && P.k > 0) {
+            some(0);
+            c = W;
         }
+        for (; c + (U - 1) * W < whole; c += U * W) {
+            Codes16 w[U][R], a[U], b[U];
 #pragma unroll
-        for (int u = 0; u < U; u++) column(w[u], a[u], b[u]);
-    }
-    for (; c * 64 < P.k; c += W) {  // the last columns, one at a time
-        const int64_t k0 = c * 64 + 16 * q;
-        uint4 w[R];
+            for (int u = 0; u < U; u++) {
+                const int64_t k0 = (c + u * W) * 64 + 16 * q;
 #pragma unroll
-        for (int r = 0; r < R; r++) w[r] = load_tail(wr[r], k0, P.k);
-        column(w, lo_in ? load_tail(xlo, k0, P.k) : zero, hi_in ? load_tail(xhi, k0, P.k) : zero);
+                for (int r = 0; r < R; r++) w[u][r].load_inside(wr[r] + k0);
+                a[u].zero();
+                b[u].zero();
+                if (lo_in) a[u].load_inside(xlo + k0);
+                if (hi_in) b[u].load_inside(xhi + k0);
+            }
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                uint4 v[R];
+#pragma unroll
+                for (int r = 0; r < R; r++) v[r] = w[u][r].codes();
+                column(v, a[u].codes(), b[u].codes());
+            }
+        }
+        for (; c * 64 < P.k; c += W) some(c);
+    } else {
+        const int64_t whole = P.k / 64;
+        int64_t c = warp;
+        for (; c + (U - 1) * W < whole; c += U * W) {
+            uint4 w[U][R], a[U], b[U];
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                const int64_t k0 = (c + u * W) * 64 + 16 * q;
+#pragma unroll
+                for (int r = 0; r < R; r++) w[u][r] = load_stream(wr[r] + k0);
+                a[u] = load_token(xlo + k0, lo_in);
+                b[u] = HI ? load_token(xhi + k0, hi_in) : zero;
+            }
+#pragma unroll
+            for (int u = 0; u < U; u++) column(w[u], a[u], b[u]);
+        }
+        for (; c * 64 < P.k; c += W) {  // the last columns, one at a time
+            const int64_t k0 = c * 64 + 16 * q;
+            uint4 w[R];
+#pragma unroll
+            for (int r = 0; r < R; r++) w[r] = load_tail(wr[r], k0, P.k);
+            column(w, lo_in ? load_tail(xlo, k0, P.k) : zero, hi_in ? load_tail(xhi, k0, P.k) : zero);
+        }
     }
 #pragma unroll
     for (int r = 0; r < R; r++)
@@ -139,13 +179,13 @@ __global__ void __launch_bounds__(W * 32, 16 / W) int8_gemv_kernel(const Int8Pro
     }
 }
 
-template <typename OT, int R, int W, int U>
+template <typename OT, int R, int W, int U, bool LOOSE>
 cudaError_t launch_gv(const Int8Product& p, cudaStream_t s) {
     const int64_t blocks = (p.n + 8 * R - 1) / (8 * R);
     if (blocks > INT32_MAX) return cudaErrorNotSupported;
     const dim3 grid((unsigned)blocks);
-    return p.m > 8 ? pipe::launch_pdl(int8_gemv_kernel<OT, R, true, W, U>, grid, W * 32, 0, s, p)
-                   : pipe::launch_pdl(int8_gemv_kernel<OT, R, false, W, U>, grid, W * 32, 0, s, p);
+    return p.m > 8 ? pipe::launch_pdl(int8_gemv_kernel<OT, R, true, W, U, LOOSE>, grid, W * 32, 0, s, p)
+                   : pipe::launch_pdl(int8_gemv_kernel<OT, R, false, W, U, LOOSE>, grid, W * 32, 0, s, p);
 }
 
 // Few rows: eight to a CTA, K over eight warps, so that every SM has a CTA (1024
@@ -153,21 +193,24 @@ cudaError_t launch_gv(const Int8Product& p, cudaStream_t s) {
 // what the tokens' rows cost (4096 x 14336: 11.6 us, eight rows 13.6), and from
 // four CTAs an SM on four warps, whose longer runs of K keep the loads flowing
 // (14336 x 4096: 11.9 us at one token and 14.2 at sixteen, eight warps 13.2 and 15.5).
+// Off the grid fewer columns are in flight: each takes twice the registers.
 template <typename OT>
 cudaError_t launch_gv_type(const Int8Product& p, cudaStream_t s) {
     const int64_t ctas16 = (p.n + 15) / 16, sms = sm_count();
-    if (ctas16 < sms) return launch_gv<OT, 1, 8, 8>(p, s);
-    return ctas16 < 4 * sms ? launch_gv<OT, 2, 8, 4>(p, s) : launch_gv<OT, 2, 4, 4>(p, s);
+    if (!int8_aligned(p))
+        return ctas16 < sms ? launch_gv<OT, 1, 8, 4, true>(p, s) : launch_gv<OT, 2, 8, 2, true>(p, s);
+    if (ctas16 < sms) return launch_gv<OT, 1, 8, 8, false>(p, s);
+    return ctas16 < 4 * sms ? launch_gv<OT, 2, 8, 4, false>(p, s) : launch_gv<OT, 2, 4, 4, false>(p, s);
 }
 
 }  // namespace
 
 cudaError_t launch_int8_gemv(const Int8Product& p, cudaStream_t s) {
-    if (p.m > 16 || !int8_aligned(p)) return cudaErrorNotSupported;
+    if (p.m > 16) return cudaErrorNotSupported;
     // the second half of the tokens' loads costs a fifth of the rate, the tile kernel 2 us more to
     // start: sixteen tokens at 28672 x 8192 46.6 us here and 40.7 there, at 14336 x 4096 13.8
     // and 12.9, at 4096 x 4096 5.6 and 7.0
-    if (p.m > 8 && p.n * p.k > 40 * 1000 * 1000) return cudaErrorNotSupported;
+    if (int8_aligned(p) && p.m > 8 && p.n * p.k > 40 * 1000 * 1000) return cudaErrorNotSupported;
     switch (p.otype) {
     case CLQ_X_F32: return launch_gv_type<float>(p, s);
     case CLQ_X_BF16: return launch_gv_type<__nv_bfloat16>(p, s);

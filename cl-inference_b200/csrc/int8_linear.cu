@@ -2,67 +2,111 @@
 //   out[t, j] = round(float(sum_c x[t, c] * w[j, c]) * (w scale j) * (x scale t) + residual[t, j])
 // with the sum in 32-bit integers, so it is exact and the same however it is
 // split.  This file holds the C entry points of the 8-bit operators, the
-// choice of a kernel, and the kernel for operands that no wide load can read.
+// choice of a kernel, and the kernel for operands off the 16-byte grid.
 #include <cstdint>
 
 #include <cuda_runtime.h>
 
 #include "../../include/clq.h"
 #include "clq_internal.h"
+#include "int8_mma.cuh"
 #include "int8_out.cuh"
+#include "launch.cuh"
+#include "pipeline.cuh"
 
 namespace clq {
 namespace {
 
-// A CTA forms 64 x 64 outputs, 4 x 4 a thread, from 32-byte columns of both
-// operands staged in shared memory a byte at a time (any base and stride),
-// four products to an instruction.
-constexpr int kGT = 64, kGK = 32;
-__global__ void __launch_bounds__(256) linear_int8_generic_kernel(const Int8Product P) {
-    __shared__ int xs[kGK / 4][kGT + 1], ws[kGK / 4][kGT + 1];
-    const int64_t n0 = (int64_t)blockIdx.x * kGT;
-    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-    for (int64_t t0 = (int64_t)blockIdx.y * kGT; t0 < P.m; t0 += (int64_t)gridDim.y * kGT) {
-        int acc[4][4] = {};
-        for (int64_t k0 = 0; k0 < P.k; k0 += kGK) {
-            for (int e = threadIdx.x; e < kGT * kGK / 4; e += 256) {
-                const int r = e / (kGK / 4), c = e % (kGK / 4);
-                uint32_t a = 0, b = 0;
-                for (int i = 0; i < 4; i++) {
-                    const int64_t kk = k0 + 4 * c + i;
-                    if (kk < P.k && t0 + r < P.m) a |= (uint32_t)(uint8_t)P.x[(t0 + r) * P.ldx + kk] << (8 * i);
-                    if (kk < P.k && n0 + r < P.n) b |= (uint32_t)(uint8_t)P.w[(n0 + r) * P.ldw + kk] << (8 * i);
-                }
-                xs[c][r] = (int)a;
-                ws[c][r] = (int)b;
+// The product for rows of any address and stride, which TMA cannot read.  A CTA
+// forms kLT tokens x kLT weight rows from 128-byte columns of both operands: 16
+// codes a load, shifted out of the two 16-byte words around them into shared memory
+// after the column before has been multiplied (their words are in flight meanwhile),
+// rows 144 bytes apart so that the eight of an ldmatrix take different banks.  Each
+// of eight warps forms 32 tokens x 16 rows with m16n8k32 integer MMAs.  Bound by L1 (83%
+// busy), which passes every word twice: 2048 x 4096 x 4096 290 us, with four bytes of
+// products to an instruction 1210, with 64-byte columns, four of them in flight, 365.
+constexpr int kLT = 64, kLK = 128, kLPitch = kLK + 16;
+__device__ __forceinline__ void load_fragments(uint32_t (&r)[4], const uint8_t* p) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"((uint32_t)__cvta_generic_to_shared(p)));
+}
+template <typename OT>
+__global__ void __launch_bounds__(256, 2) int8_loose_kernel(const Int8Product P) {
+    __shared__ __align__(16) uint8_t sh[2][2][kLT][kLPitch];  // [column parity][tokens, rows]
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int row = tid >> 3, chunk = tid & 7;  // staged: rows row and row + 32 of both, 16 codes each
+    const int wt = (warp >> 2) * 32, wn = (warp & 3) * 16;
+    const int64_t n0 = (int64_t)blockIdx.x * kLT, columns = (P.k + kLK - 1) / kLK;
+    pipe::grid_dependency_wait();
+    pipe::allow_dependents();
+    for (int64_t t0 = (int64_t)blockIdx.y * kLT; t0 < P.m; t0 += (int64_t)gridDim.y * kLT) {
+        const int8_t* src[4];
+#pragma unroll
+        for (int i = 0; i < 2; i++) {  // rows past the last repeat it and are not written
+            src[i] = P.x + min(t0 + row + 32 * i, P.m - 1) * P.ldx;
+            src[2 + i] = P.w + min(n0 + row + 32 * i, P.n - 1) * P.ldw;
+        }
+        Codes16 next[4];
+        const auto fetch = [&](int64_t c) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) next[i].load(src[i], c * kLK + 16 * chunk, P.k);
+        };
+        const auto stage = [&](int64_t c) {
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                *reinterpret_cast<uint4*>(&sh[c & 1][i >> 1][row + 32 * (i & 1)][16 * chunk]) = next[i].codes();
+        };
+        int acc[2][2][4] = {};
+        if (columns > 0) {
+            fetch(0);
+            stage(0);
+        }
+        __syncthreads();
+        for (int64_t c = 0; c < columns; c++) {
+            if (c + 1 < columns) fetch(c + 1);
+            const auto& tokens = sh[c & 1][0];
+            const auto& rows = sh[c & 1][1];
+#pragma unroll
+            for (int kk = 0; kk < kLK; kk += 32) {
+                uint32_t a[2][4], b[4];
+#pragma unroll
+                for (int i = 0; i < 2; i++) load_fragments(a[i], &tokens[wt + 16 * i + (lane & 15)][kk + 16 * (lane >> 4)]);
+                load_fragments(b, &rows[wn + (lane & 7) + 8 * (lane >> 4)][kk + 16 * (lane >> 3 & 1)]);
+#pragma unroll
+                for (int i = 0; i < 2; i++)
+#pragma unroll
+                    for (int j = 0; j < 2; j++)
+                        mma_s8(acc[i][j], a[i][0], a[i][1], a[i][2], a[i][3], b[2 * j], b[2 * j + 1]);
             }
-            __syncthreads();
-#pragma unroll
-            for (int c = 0; c < kGK / 4; c++)
-#pragma unroll
-                for (int i = 0; i < 4; i++)
-#pragma unroll
-                    for (int j = 0; j < 4; j++) acc[i][j] = __dp4a(xs[c][ty + 16 * i], ws[c][tx + 16 * j], acc[i][j]);
+            if (c + 1 < columns) stage(c + 1);  // the other buffer: read before the last barrier
             __syncthreads();
         }
-        for (int i = 0; i < 4; i++)
-            for (int j = 0; j < 4; j++) {
-                const int64_t t = t0 + ty + 16 * i, n = n0 + tx + 16 * j;
-                if (t >= P.m || n >= P.n) continue;
-                float v = int8_scaled(acc[i][j], P.ws[n], P.xs[t]);
-                if (P.res) v = __fadd_rn(v, P.res[t * P.ldr + n]);
-                if (P.otype == CLQ_X_F32) static_cast<float*>(P.out)[t * P.ldo + n] = v;
-                else if (P.otype == CLQ_X_BF16) static_cast<__nv_bfloat16*>(P.out)[t * P.ldo + n] = int8_round<__nv_bfloat16>(v);
-                else static_cast<__half*>(P.out)[t * P.ldo + n] = int8_round<__half>(v);
-            }
+#pragma unroll
+        for (int i = 0; i < 2; i++)
+#pragma unroll
+            for (int j = 0; j < 2; j++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const int64_t t = t0 + wt + 16 * i + (lane >> 2) + 8 * (e >> 1), n = n0 + wn + 8 * j + 2 * (lane & 3) + (e & 1);
+                    if (t >= P.m || n >= P.n) continue;
+                    float v = int8_scaled(acc[i][j][e], P.ws[n], P.xs[t]);
+                    if (P.res) v = __fadd_rn(v, P.res[t * P.ldr + n]);
+                    static_cast<OT*>(P.out)[t * P.ldo + n] = int8_round<OT>(v);
+                }
     }
 }
 
-cudaError_t launch_linear_int8_generic(const Int8Product& p, cudaStream_t s) {
-    const int64_t bx = (p.n + kGT - 1) / kGT, by = (p.m + kGT - 1) / kGT;
-    if (bx > INT32_MAX || by > INT32_MAX) return cudaErrorInvalidConfiguration;
-    linear_int8_generic_kernel<<<dim3((unsigned)bx, (unsigned)(by < 65535 ? by : 65535)), 256, 0, s>>>(p);
-    return cudaGetLastError();
+cudaError_t launch_int8_loose(const Int8Product& p, cudaStream_t s) {
+    const int64_t bx = (p.n + kLT - 1) / kLT, by = (p.m + kLT - 1) / kLT;
+    if (bx > INT32_MAX) return cudaErrorInvalidConfiguration;
+    const dim3 grid((unsigned)bx, (unsigned)(by < 65535 ? by : 65535));
+    switch (p.otype) {
+    case CLQ_X_F32: return pipe::launch_pdl(int8_loose_kernel<float>, grid, 256, 0, s, p);
+    case CLQ_X_BF16: return pipe::launch_pdl(int8_loose_kernel<__nv_bfloat16>, grid, 256, 0, s, p);
+    case CLQ_X_F16: return pipe::launch_pdl(int8_loose_kernel<__half>, grid, 256, 0, s, p);
+    default: return cudaErrorInvalidValue;
+    }
 }
 
 int i8_fail(int code, const char* what) { return set_error(code, "%s", what); }
@@ -99,10 +143,9 @@ bool int8_aligned(const Int8Product& p) {
 }
 
 cudaError_t launch_linear_int8(const Int8Product& p, cudaStream_t s) {
-    if (p.k < 1 || !int8_aligned(p)) return launch_linear_int8_generic(p, s);
     cudaError_t e = launch_int8_gemv(p, s);
     if (e == cudaErrorNotSupported) e = launch_int8_gemm(p, s);
-    return e == cudaErrorNotSupported ? launch_linear_int8_generic(p, s) : e;
+    return e == cudaErrorNotSupported ? launch_int8_loose(p, s) : e;
 }
 
 }  // namespace clq

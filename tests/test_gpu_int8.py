@@ -365,6 +365,26 @@ def test_linear_of_unaligned_rows(cuda, clq, m, what):
     check_product(torch, clq.linear_int8(x, w), x, w)
 
 
+@pytest.mark.parametrize("m", [1, 7, 8, 9, 16, 17, 64, 65, 200])
+@pytest.mark.parametrize("n,k", [(1, 1), (5, 15), (9, 16), (64, 17), (65, 31), (33, 47), (20, 63), (150, 79), (16, 80), (31, 95),
+                                 (130, 127), (70, 143), (64, 145), (2500, 500), (1000, 1100), (300, 2051)])
+@pytest.mark.parametrize("xoff,woff", [(1, 2), (15, 0), (4, 11)])
+def test_linear_of_rows_that_end_beside_others(cuda, clq, m, n, k, xoff, woff):
+    """Every distance from the 16-byte grid (odd strides), the neighbours' codes not taken in, the
+    first row at its buffer's start and the last at its end."""
+    torch = cuda
+
+    def rows(count, off, seed):
+        c, s = codes_of(torch, 1, count * k + off, seed, pitch=count * k + off)
+        return clq.Int8Rows(c[0, off:].view(count, k), s.expand(count).contiguous())
+    x, w = rows(m, xoff, 1), rows(n, woff, 2)
+    res = rand(torch, m, n, seed=3)
+    check_product(torch, clq.linear_int8(x, w, dtype=torch.bfloat16, residual=res), x, w, res)
+    exact = x.codes.double() @ w.codes.double().t()
+    ones = [clq.Int8Rows(q.codes, torch.ones_like(q.scales)) for q in (x, w)]
+    assert torch.equal(clq.linear_int8(*ones).double(), exact.float().double())
+
+
 @pytest.mark.parametrize("m", [1, 6, 16, 40, 130, 300])
 @pytest.mark.parametrize("dtype", TYPES)
 def test_linear_into_a_wider_buffer_and_onto_its_residual(cuda, clq, m, dtype):
