@@ -338,10 +338,10 @@ int clq_attend_device(const float *q, int64_t count, int n_heads, int64_t q_pos_
 
 /* ---- 8-bit activations ------------------------------------------------------
  * No counterpart in the reference (its activations are f32).  Rows of int8
- * codes with one f32 scale a row, value = code * scale, made with the rule of
- * the Q8 cache codec over the whole row: step = max(FLT_MIN, peak / 127), code =
- * clamp(round-half-even(v / step), -127, 127), the quotient formed as a product
- * with the rounded 1 / step; an all-zero row has the scale 1, and a row with a
+ * codes with one f32 scale a row, value = code * scale: step = max(FLT_MIN, peak /
+ * 127), code = clamp(round-half-even(v * inv), -127, 127) with inv = 1 / step, every
+ * quotient and product rounded to f32 (the step of the Q8 cache codec over the
+ * whole row; that codec divides by it).  An all-zero row has the scale 1, and a row with a
  * non-finite value has codes 0 and the scale NaN.  Row strides are in elements;
  * each row is contiguous.  Any address that its element type allows is taken
  * (others are CLQ_ERR_ARGUMENT); code rows that start on 16-byte boundaries (base
