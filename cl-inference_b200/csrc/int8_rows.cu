@@ -39,17 +39,18 @@ __device__ __forceinline__ float to_f32(float v) { return v; }
 __device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
 __device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
 
-// silu(g) * u = g / (1 + 2^(-g log2 e)) * u.  The exponent's product is kept in
-// two parts (t and what its rounding left), so that the relative error stays that
-// of ex2.approx (2^-22) for every gate; with rcp.approx (2^-23) and four f32
-// roundings v is within 10 roundings of 2^-24, where the library's exponential and
-// an IEEE quotient have 7 and cost three times the instructions, which bound this
-// kernel (2048 rows of 14336 bf16: 235 us in the first form, 35 now).  Gates
-// below -87 count as -87 in the quotient, whose value there is under 2^-125.  A
-// gate that is not finite stays so: v becomes NaN or infinite.
-__device__ __forceinline__ float silu_times(float g, float u) {
+// silu(g) * u = g / (1 + 2^(-g log2 e)) * u for gates from kFarGate, where the power and
+// the reciprocal stay normal numbers (below, anything).  The exponent's product is kept
+// in two parts (t and what its rounding left), so that the relative error stays that of
+// ex2.approx (2^-22); with rcp.approx (2^-23) and four f32 roundings v is within 10
+// roundings of 2^-24.  The library's exponential and an IEEE quotient have 7, and take
+// the kernel, which instructions bound, from 36 us to 58 (2048 rows of 14336 bf16, where
+// 4 codes of 29 million then differ).  A gate that is NaN or infinite gives NaN or an
+// infinity.
+constexpr float kFarGate = -87.f;
+__device__ __forceinline__ float silu_near(float g, float u) {
     constexpr float kLog2e = 1.44269504f, kLog2eLow = 1.92596303e-8f, kLn2 = 0.693147181f;
-    const float n = -fminf(fmaxf(g, -87.f), 200.f);
+    const float n = -fminf(g, 200.f);
     const float t = __fmul_rn(n, kLog2e);
     const float low = fmaf(n, kLog2eLow, fmaf(n, kLog2e, -t));
     float e, r;
@@ -57,6 +58,34 @@ __device__ __forceinline__ float silu_times(float g, float u) {
     const float d = 1.f + fmaf(e, low * kLn2, e);
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d));
     return __fmul_rn(__fmul_rn(g, r), u);
+}
+// And below, where 1 + e^-g is e^-g to f32 and may leave it: g e^g u, the power as two
+// factors around u, so that a gate's tail times a large u is kept: within 11 roundings
+// (two of the exponential's 2^-22 and three products) and, past -174, where e^(g/2) is
+// subnormal, 2^-137 for any u.  -infinity gives NaN.
+__device__ __forceinline__ float silu_far(float g, float u) {
+    const float h = expf(0.5f * g);
+    return __fmul_rn(__fmul_rn(__fmul_rn(g, h), u), h);
+}
+// V values of it over the u, the far gates behind one branch: a step seldom holds any
+// (2048 x 14336 bf16 36.4 us; 38.0 with selects in every element, 37.6 with one branch
+// after a thread's whole share).
+template <int V>
+__device__ __forceinline__ void silu_times(const float (&g)[V], float (&u)[V]) {
+    bool far = false;
+    float v[V];
+#pragma unroll
+    for (int j = 0; j < V; j++) {
+        far = far || g[j] < kFarGate;
+        v[j] = silu_near(g[j], u[j]);
+    }
+    if (far) {
+#pragma unroll
+        for (int j = 0; j < V; j++)
+            if (g[j] < kFarGate) v[j] = silu_far(g[j], u[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < V; j++) u[j] = v[j];
 }
 
 // max(a, |v|), NaN once either is.
@@ -68,16 +97,19 @@ __device__ __forceinline__ float peak_of(float a, float v) {
 
 enum { kPlain, kNorm, kSwiglu };
 
-// v and, for a norm, the sum of squares of h.
-template <int MODE>
-__device__ __forceinline__ float value_of(float x, float other, float w, float& ss) {
-    if constexpr (MODE == kSwiglu) return silu_times(other, x);
-    const float h = __fadd_rn(x, other);
-    if constexpr (MODE == kNorm) {
-        ss = fmaf(h, h, ss);
-        return __fmul_rn(h, w);
+// V values of v in place of X's, the peak and, for a norm, the sum of squares of h.
+template <int MODE, int V>
+__device__ __forceinline__ void values_of(float (&x)[V], const float (&other)[V], const float (&w)[V], float& ss, float& peak) {
+    if constexpr (MODE == kSwiglu) silu_times(other, x);
+#pragma unroll
+    for (int j = 0; j < V; j++) {
+        if constexpr (MODE != kSwiglu) x[j] = __fadd_rn(x[j], other[j]);
+        if constexpr (MODE == kNorm) {
+            ss = fmaf(x[j], x[j], ss);
+            x[j] = __fmul_rn(x[j], w[j]);
+        }
+        peak = peak_of(peak, x[j]);
     }
-    return h;
 }
 
 struct RowScale {
@@ -284,11 +316,7 @@ __global__ void __launch_bounds__(G == 32 ? kSmallRow : G, min_ctas<XT, step_of<
             if constexpr (MODE == kNorm) {
                 if (i < k) load_values<float, V>(Q.norm_w + i, w);
             }
-#pragma unroll
-            for (int j = 0; j < V; j++) {
-                v[c0 + b][j] = value_of<MODE>(v[c0 + b][j], o[j], w[j], ss);
-                peak = peak_of(peak, v[c0 + b][j]);
-            }
+            values_of<MODE>(v[c0 + b], o, w, ss, peak);
         }
     }
     const float2 sums = G == 32 ? row_reduce_warp(ss, peak) : row_reduce_cta(ss, peak, red, G / 32);
@@ -542,11 +570,7 @@ __global__ void __launch_bounds__(stream_threads(LOOSE), !LOOSE && C * 16 / (int
                 if constexpr (LOOSE) store_shifted<RT, V>(res_out, i, k, h);
                 else if (i < k) store_values<RT, V>(res_out + i, h);
             }
-#pragma unroll
-            for (int j = 0; j < V; j++) {
-                v[c][j] = value_of<MODE>(v[c][j], ov[j], w[j], ss);
-                peak = peak_of(peak, v[c][j]);
-            }
+            values_of<MODE>(v[c], ov, w, ss, peak);
         }
         const float2 sums = row_reduce_cta(ss, peak, red + turn * (kStreamThreads / 32), G / 32);
         if (tid < 32) issue(next, s, false);
@@ -595,8 +619,13 @@ __global__ void __launch_bounds__(kLongThreads) quantize_long_rows_kernel(const 
     RT* res_out = Q.res_out ? static_cast<RT*>(Q.res_out) + row * Q.ldro : nullptr;
     const auto other = [&](int64_t i) { return MODE == kSwiglu ? to_f32(gate[i]) : res ? to_f32(res[i]) : -0.f; };
     float ss = 0.f, peak = 0.f;
-    for (int64_t i = threadIdx.x; i < Q.k; i += kLongThreads)
-        peak = peak_of(peak, value_of<MODE>(to_f32(x[i]), other(i), MODE == kNorm ? Q.norm_w[i] : 0.f, ss));
+    const auto value = [&](float a, float o, int64_t i) {
+        float v[1] = {a};
+        const float others[1] = {o}, w[1] = {MODE == kNorm ? Q.norm_w[i] : 0.f};
+        values_of<MODE>(v, others, w, ss, peak);
+        return v[0];
+    };
+    for (int64_t i = threadIdx.x; i < Q.k; i += kLongThreads) value(to_f32(x[i]), other(i), i);
     const float2 sums = row_reduce_cta(ss, peak, red, kLongThreads / 32);
     const RowScale r = row_scale<MODE>(Q, sums.x, sums.y);
     if (threadIdx.x == 0) Q.scales[row] = r.scale;
@@ -604,7 +633,7 @@ __global__ void __launch_bounds__(kLongThreads) quantize_long_rows_kernel(const 
     for (int64_t i = threadIdx.x; i < Q.k; i += kLongThreads) {
         const float a = to_f32(x[i]), o = other(i);
         if (MODE != kSwiglu && res_out) res_out[i] = int8_round<RT>(__fadd_rn(a, o));
-        const float v = value_of<MODE>(a, o, MODE == kNorm ? Q.norm_w[i] : 0.f, ss);
+        const float v = value(a, o, i);
         codes[i] = r.inv > 0.f ? (int8_t)code_bits(v, r.inv) : (int8_t)0;
     }
 }

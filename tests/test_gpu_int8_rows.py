@@ -42,3 +42,69 @@ def test_codes_follow_the_documented_product(cuda, clq, m, k):
               clq.norm_quantize(zero, None, residual=d)[0]):
         assert np.array_equal(q.codes.cpu().numpy(), want.astype(np.int8))
     assert np.array_equal(clq.quantize_rows(d).scales.cpu().numpy(), step[:, 0])
+
+
+def far_gates(torch, m, k, xtype):
+    """(gate, up) whose rows lie, or mostly lie, where e^-gate leaves f32."""
+    gen = torch.Generator(device="cuda").manual_seed(m + k)
+
+    def uniform(low, high):
+        return torch.rand(m, k, device="cuda", generator=gen, dtype=torch.float64) * (high - low) + low
+    most = 4.0 if xtype == "float16" else 38.0  # decimal exponents of up
+    gate, up = uniform(-220, -87), 10 ** uniform(-2, most) * torch.sign(uniform(-1, 1))
+    few = torch.tensor([-88.0, -95.0, -120.0, -300.0], dtype=torch.float64, device="cuda")
+    for r in range(m):
+        kind = r % 6
+        if kind == 1:  # the smallest value must not lead the row
+            gate[r] = few.repeat(k // 4 + 1)[:k]
+            up[r] = torch.arange(1.0, 5.0, device="cuda", dtype=torch.float64).repeat(k // 4 + 1)[:k]
+        elif kind == 2:  # as far as the type goes, beside one value of the row's kind above
+            gate[r] = -60000.0 if xtype == "float16" else torch.where(uniform(0, 1)[r] < 0.5, -1e30, -3e38)
+            gate[r, k // 2] = -88.0
+            up[r] = 10.0 ** most
+        elif kind == 3:  # beside values of ordinary size
+            gate[r, k // 3:] = uniform(-3, 3)[r, k // 3:]
+            gate[r, :k // 3] = -60000.0 if xtype == "float16" else -1e38
+            up[r] = uniform(-2, 2)[r]
+            gate[r, k - 1], up[r, k - 1] = 1.5, 1.0
+        elif kind == 4:  # both sides of where the formula changes
+            gate[r], up[r] = uniform(-87.5, -86.5)[r], uniform(1, 2)[r]
+        elif kind == 5:  # results about the smallest normal number and below it
+            gate[r], up[r] = uniform(-200, -170)[r], 10.0 ** most
+    dtype = getattr(torch, xtype)
+    return gate.to(dtype), up.to(dtype)
+
+
+@pytest.mark.parametrize("m,k", [(6, 4), (6, 96), (12, 1001), (6, 4096), (6, 4099), (160, 5003), (600, 2048), (600, 9000),
+                                 (300, 9001), (6, 40000)])
+@pytest.mark.parametrize("xtype", ["float32", "bfloat16", "float16"])
+def test_swiglu_of_rows_of_far_gates(cuda, clq, m, k, xtype):
+    """Gates below -87, where silu decays to 0 however large they are, lead or share a row.
+    v is within 11 U and 2^-137 of the exact value (include/clq.h), the peak too, peak / 127,
+    1 / step and the product round once each: a code is within 127 * 25 U of the quotient and, as a step
+    has FLT_MIN at least, 2^-137 / 2^-126 twice more; the scale within 12 U and 2^-137 / 127, and the
+    half of a smallest number where it is FLT_MIN or less."""
+    torch = cuda
+    gate, up = far_gates(torch, m, k, xtype)
+    q = clq.swiglu_quantize(gate, up)
+    g = gate.double()
+    v = g * torch.sigmoid(g) * up.double()
+    assert torch.isfinite(v).all()
+    peak = v.abs().amax(1)
+    assert (peak > 0).all()
+    step = torch.clamp(peak / 127, min=2.0 ** -126)
+    # a peak under the bound may come out as 0 or not: a row of zeros has scale 1, and codes 0 like the other
+    nothing = (peak <= 2.0 ** -137) & (q.scales == 1)
+    assert (((q.scales.double() - step).abs() <= 12 * U * step + 2.0 ** -137) | nothing).all()
+    ideal = (v / step[:, None]).clamp(-127, 127)
+    assert ((q.codes.double() - ideal).abs() <= 0.5 + 127 * 25 * U + 2 * 2.0 ** -11).all()
+
+
+def test_gates_that_are_not_finite(cuda, clq):
+    torch = cuda
+    for k in (8, 4097, 40000):
+        gate = torch.full((4, k), -90.0, device="cuda")
+        up = torch.ones(4, k, device="cuda")
+        gate[0, k - 1], gate[1, 0], gate[2, k // 2] = float("-inf"), float("nan"), float("inf")
+        q = clq.swiglu_quantize(gate, up)
+        assert torch.isnan(q.scales[:3]).all() and not q.codes[:3].any() and q.scales[3].item() == 2.0 ** -126
