@@ -15,8 +15,8 @@
 // together) serves both, and a row is read once, its values held in registers
 // between the reduction and the rounding.  Bound by memory for many rows and by
 // one round trip and the reduction for few.  A row that holds a non-finite h or v, or whose sum of
-// squares leaves f32, gets codes 0 and the scale NaN, so that every product
-// formed with it is NaN.
+// squares leaves f32 at either end, gets codes 0 and the scale NaN, so that every
+// product formed with it is NaN.
 #include <atomic>
 #include <cfloat>
 #include <cstdint>
@@ -120,8 +120,11 @@ __device__ __forceinline__ RowScale row_scale(const QuantRows& Q, float ss, floa
     bool fine = peak < INFINITY;  // not NaN either
     float s = 1.f;
     if constexpr (MODE == kNorm) {
-        s = __fdiv_rn(1.f, __fsqrt_rn(__fdiv_rn(ss, (float)Q.k) + Q.eps));
-        fine = fine && ss < INFINITY;
+        // Squares under 2^-126 lose bits, 2^-150 of the mean at most and as much in its
+        // rounding: no more than 2^-24 of a sum with eps that reaches 2^-125.
+        const float mean = __fadd_rn(__fdiv_rn(ss, (float)Q.k), Q.eps);
+        s = __fdiv_rn(1.f, __fsqrt_rn(mean));
+        fine = fine && ss < INFINITY && (mean >= 2.f * FLT_MIN || peak == 0.f);
     }
     const float step = fmaxf(FLT_MIN, __fdiv_rn(peak, 127.f));
     RowScale r;

@@ -188,6 +188,8 @@ def norm_quantize(x, norm_weight=None, eps=1e-5, residual=None, residual_out=Non
     Without NORM_WEIGHT (f32 [k]) the sum itself is coded; without RESIDUAL (x's
     type, or f32) x alone.  With a residual returns (rows, x + residual), the sum
     in the residual's type: RESIDUAL_OUT, which may be RESIDUAL, or a new tensor.
+    A row that is not finite, or whose mean square + EPS is not within f32 (from 2^-125
+    on), has codes 0 and the scale NaN.
     """
     torch = _t or _torch()
     if stream is not None:

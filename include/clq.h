@@ -357,7 +357,8 @@ int clq_quantize_rows_device(const void *x, int xtype, int64_t m, int64_t k, int
  * (the residual addition of layer-forward, local/blocks.lisp:387-392, and the
  * apply-rmsnorm of the next block, :115-116).  RESIDUAL, RESIDUAL_OUT and NORM_WEIGHT (f32 [K]; without it h itself is coded) may be
  * null.  RTYPE, of both residuals, is XTYPE or CLQ_X_F32.  A row whose sum of
- * squares leaves f32 counts as non-finite. */
+ * squares leaves f32 counts as non-finite: upwards, or with mean(h^2) + norm_epsilon under
+ * 2^-125 (an epsilon of 0, say, and |h| about 1e-19) unless all of its codes are of zeros. */
 int clq_norm_quantize_device(const void *x, int xtype, int64_t m, int64_t k, int64_t ldx, const float *norm_weight,
                              float norm_epsilon, const void *residual, int rtype, int64_t ldr, void *residual_out,
                              int64_t ldro, int8_t *codes, int64_t ldc, float *scales, void *stream);

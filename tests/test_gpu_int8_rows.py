@@ -108,3 +108,31 @@ def test_gates_that_are_not_finite(cuda, clq):
         gate[0, k - 1], gate[1, 0], gate[2, k // 2] = float("-inf"), float("nan"), float("inf")
         q = clq.swiglu_quantize(gate, up)
         assert torch.isnan(q.scales[:3]).all() and not q.codes[:3].any() and q.scales[3].item() == 2.0 ** -126
+
+
+@pytest.mark.parametrize("k", [16, 100, 4096, 5001, 40000])
+@pytest.mark.parametrize("rtype", ["float32", "bfloat16"])
+def test_norm_of_small_rows_without_epsilon(cuda, clq, k, rtype):
+    """Where the squares leave f32 downwards the scale is NaN as it is upwards, never infinite; above
+    2^-125 it is right: the sum of squares within (k / 32 + 24) U as for any row and 2^-24 for what
+    squares lost, halved by the root, and 20 U for the steps around it."""
+    torch = cuda
+    gen = torch.Generator(device="cuda").manual_seed(k)
+    sign = torch.sign(torch.randn(8, k, device="cuda", generator=gen))
+    sizes = [2.0 ** -62, 2.0 ** -64, 1e-25, 1e-38, 2.0 ** -133, 1.0, 0.0, 2.0 ** -61.5]
+    h = (sign * torch.tensor(sizes, device="cuda")[:, None]).to(getattr(torch, rtype))
+    zero = torch.zeros(8, k, device="cuda", dtype=torch.bfloat16)
+    g = torch.ones(k, device="cuda")
+    for q in (clq.norm_quantize(h, g, 0.0), clq.norm_quantize(zero, g, 0.0, residual=h)[0], clq.norm_quantize(h, g, 1e-44)):
+        for row in (1, 2, 3, 4):
+            assert torch.isnan(q.scales[row]) and not q.codes[row].any(), row
+        assert q.scales[6].item() == 1.0 and not q.codes[6].any()
+        for row in (0, 5, 7):
+            d = h[row].double()
+            want = d.abs().max() / 127 / torch.sqrt((d * d).mean())
+            assert abs(q.scales[row].double() / want - 1).item() <= (k / 64 + 33) * U
+            assert torch.equal(q.codes[row].float(), 127 * sign[row])
+    fine = clq.norm_quantize(h, g, 1e-5)
+    assert torch.isfinite(fine.scales).all()
+    # a weight of zeros leaves nothing to code: an all-zero row
+    assert (clq.norm_quantize(h, 0 * g, 0.0).scales == 1).all()
