@@ -336,6 +336,9 @@ __global__ void __launch_bounds__(G == 32 ? kSmallRow : G, min_ctas<XT, step_of<
 
 // ---- many rows, streamed through shared memory ------------------------------
 
+// In a peak's place, from a thread whose wait for its row gave up: every thread of the CTA
+// then finds it in the reduced peak (the bits are above those of any peak, NaN included).
+constexpr uint32_t kGaveUp = 0xffffffffu;
 constexpr int kStreamStages = 4;
 constexpr int kStreamHeader = 1024;  // barriers and two rows' reductions
 // Threads of a CTA at most: rows off the grid, whose reads are longer, gain by more
@@ -527,13 +530,14 @@ __global__ void __launch_bounds__(stream_threads(LOOSE), !LOOSE && C * 16 / (int
         }
     }
     __syncthreads();
-    bool ok = true;  // after a wait that gave up the rows' results are invalid, as the status word says
     int s = 0, turn = 0;
     uint32_t parity = 0;
     for (int64_t row = blockIdx.x; row < Q.m; row += gridDim.x, turn ^= 1) {
         const int64_t next = row + (int64_t)stages * gridDim.x;
         fetch_ends(next);
-        ok = pipe::mbar_wait(&full[s], parity, err) && ok;
+        // without it, the values formed below are of whatever the buffer holds, and not used
+        bool here = pipe::mbar_wait(&full[s], parity, err);
+        if (LOOSE && MODE != kSwiglu) here = __all_sync(0xffffffffu, here);  // store_shifted takes whole warps
         const auto x = x_row(row, s);
         const auto o = o_row(two ? row : 0, s);
         RT* res_out = Q.res_out ? static_cast<RT*>(Q.res_out) + row * Q.ldro : nullptr;
@@ -566,7 +570,7 @@ __global__ void __launch_bounds__(stream_threads(LOOSE), !LOOSE && C * 16 / (int
                     }
                 }
             }
-            if (MODE != kSwiglu && res_out) {
+            if (MODE != kSwiglu && res_out && here) {
                 float h[V];
 #pragma unroll
                 for (int j = 0; j < V; j++) h[j] = __fadd_rn(v[c][j], ov[j]);
@@ -575,7 +579,16 @@ __global__ void __launch_bounds__(stream_threads(LOOSE), !LOOSE && C * 16 / (int
             }
             values_of<MODE>(v[c], ov, w, ss, peak);
         }
+        if (!here) peak = __uint_as_float(kGaveUp);
         const float2 sums = row_reduce_cta(ss, peak, red + turn * (kStreamThreads / 32), G / 32);
+        if (__float_as_uint(sums.y) == kGaveUp) {
+            // nothing more is copied, read or written; what is in flight lands before the CTA exits
+            for (int i = 0; tid == 0 && i < stages && row + (int64_t)i * gridDim.x < Q.m; i++) {
+                const bool wrapped = s + i >= stages;
+                pipe::mbar_drain(&full[wrapped ? s + i - stages : s + i], parity ^ (wrapped ? 1u : 0u));
+            }
+            return;
+        }
         if (tid < 32) issue(next, s, false);
         if (LOOSE && stages == 1) __syncthreads();  // the ends just written are read in the next turn
         if (++s == stages) {
@@ -598,11 +611,6 @@ __global__ void __launch_bounds__(stream_threads(LOOSE), !LOOSE && C * 16 / (int
             }
         }
     }
-    if (!ok && tid == 0)
-        for (int i = 0; i < stages; i++) {  // what is in flight lands before the CTA exits
-            pipe::mbar_drain(&full[i], 0);
-            pipe::mbar_drain(&full[i], 1);
-        }
 }
 
 // ---- rows longer than the registers of a CTA hold --------------------------
