@@ -78,6 +78,11 @@ __device__ __forceinline__ int4 load_cluster(uint32_t addr) {
                  : "memory");
     return v;
 }
+__device__ __forceinline__ uint32_t load_cluster_u32(uint32_t addr) {
+    uint32_t v;
+    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+    return v;
+}
 __device__ __forceinline__ void arrive_cluster(uint32_t bar) {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
@@ -123,6 +128,10 @@ __device__ __forceinline__ void mma_commit(uint32_t bar) {
             "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
             "h"((uint16_t)3)
             : "memory");
+}
+// On BAR of this CTA alone.
+__device__ __forceinline__ void mma_commit_here(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
 template <int CG>
 __device__ __forceinline__ void tmem_alloc(uint32_t* slot, uint32_t cols) {
@@ -359,7 +368,7 @@ constexpr int tile_stages(int tn, int per_sm) {
     return per_sm == 2 ? (tn == 64 ? 4 : 5) : tn == 256 ? 4 : tn == 128 ? 7 : tn == 64 ? 9 : 8;
 }
 constexpr size_t tile_smem(int tn, int stages) {
-    return 1024 + (size_t)stages * (kABytes + (size_t)tn * kKB) + (2 * stages + 2) * 8 + (size_t)tn * 4;
+    return 1024 + (size_t)stages * (kABytes + (size_t)tn * kKB) + (2 * stages + 3) * 8 + (size_t)tn * 4;
 }
 constexpr bool tile_fits(int tn, int per_sm) {  // with the 1 KB that the system takes of each CTA's share
     return tile_smem(tn, tile_stages(tn, per_sm)) <= (kSmemPerSm + 1024) / per_sm - 1024 &&
@@ -371,7 +380,8 @@ static_assert(tile_fits(256, 1) && tile_fits(128, 1) && tile_fits(64, 1) && tile
 // CTA (blockIdx.x = row tile x SPLITS + part, blockIdx.y = token tile); the
 // SPLITS parts of a tile form a cluster.  Each part leaves its sums in its own
 // shared memory, over the stages it has done with, as [token][row], and part r
-// finishes the tokens [r TN / SPLITS, (r + 1) TN / SPLITS) from all of them.
+// finishes the tokens [r TN / SPLITS, (r + 1) TN / SPLITS) from all of them.  A part whose
+// sums are not whole says so beside them, and none of the tile is written.
 template <typename OT, int TN>
 __global__ void __launch_bounds__(kThreads) int8_tile_kernel(const __grid_constant__ GemmI8 G, int splits) {
     extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -382,8 +392,10 @@ __global__ void __launch_bounds__(kThreads) int8_tile_kernel(const __grid_consta
     int* sums = reinterpret_cast<int*>(A);
     uint64_t* full = reinterpret_cast<uint64_t*>(B + (size_t)NS * kBBytes);
     uint64_t* empty = full + NS;
-    uint64_t* done = empty + NS;
-    uint32_t* slot = reinterpret_cast<uint32_t*>(done + 1);
+    uint64_t* done = empty + NS;  // the sums are whole
+    uint64_t* last = done + 1;    // or, after a wait that gave up, the MMAs issued have ended
+    uint32_t* slot = reinterpret_cast<uint32_t*>(last + 1);
+    uint32_t* gave_up = slot + 1;
     float* xs = reinterpret_cast<float*>(slot + 2);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -393,10 +405,11 @@ __global__ void __launch_bounds__(kThreads) int8_tile_kernel(const __grid_consta
     const Int8Product& P = G.p;
 
     if (warp == 5) {
-        if (lane < 2 * NS + 1) mbar_init(full + lane, 1);  // full, empty, done
+        if (lane < 2 * NS + 2) mbar_init(full + lane, 1);  // full, empty, done, last
         mbar_init_fence();
     } else if (warp == 4) {
         if (lane < 2) prefetch_map(lane ? &G.xmap : &G.wmap);
+        if (lane == 2) *gave_up = 0;
     } else if (warp == 0) {
         tmem_alloc<1>(slot, TN);
     }
@@ -432,9 +445,9 @@ __global__ void __launch_bounds__(kThreads) int8_tile_kernel(const __grid_consta
         const uint32_t a0 = desc_low(smem_u32(A)), b0 = desc_low(smem_u32(B));
         constexpr uint32_t idesc = instr_desc_i8(kRows, TN);
         Ring r(NS);
-        bool ready = false;
+        bool whole = true, ready = false;
         for (int it = 0; it < nk; it++, r.next()) {
-            if (!wait_spin(fulls + 8 * r.s, r.parity(), G.err, ready)) break;
+            if (!(whole = wait_spin(fulls + 8 * r.s, r.parity(), G.err, ready))) break;
             const Ring next = r.after();
             ready = peek(fulls + 8 * next.s, next.parity());
             tc_fence_after();
@@ -444,9 +457,10 @@ __global__ void __launch_bounds__(kThreads) int8_tile_kernel(const __grid_consta
             }
             __syncwarp();
         }
-        if (elect_one()) mma_commit<1>(smem_u32(done));
+        uint64_t* ended = whole ? done : last;
+        if (elect_one()) mma_commit<1>(smem_u32(ended));
         __syncwarp();
-        mbar_drain(done, 0);
+        mbar_drain(ended, 0);
     } else {
         for (int i = threadIdx.x; i < TN; i += 128) xs[i] = t0 + i < P.m ? P.xs[t0 + i] : 0.f;
         named_sync(1, 128);
@@ -480,9 +494,11 @@ __global__ void __launch_bounds__(kThreads) int8_tile_kernel(const __grid_consta
                 for (int j = 0; j < 32; j++) sums[(c + j) * kRows + 32 * warp + lane] = v[j];
             }
         }
+        if (warp < 4 && !ok && lane == 0) *gave_up = 1;
         __syncwarp();
         cluster_arrive();
         cluster_wait();
+        if (warp < 4) ok = !__any_sync(0xffffffffu, lane < splits && load_cluster_u32(map_rank(smem_u32(gave_up), (uint32_t)lane)));
         if (ok) {
             const int c0 = TN * part / splits, c1 = min(cols, TN * (part + 1) / splits);
             const uint32_t base = smem_u32(sums) + 16 * lane;
@@ -522,7 +538,7 @@ constexpr int kPairTokens = 256, kGroup = 8;
 constexpr uint32_t kPairB = kPairTokens / 2 * kKB;  // each CTA stages half of the tokens
 constexpr uint32_t kPairRing = 6 * (kABytes + kPairB);  // six stages, or up to ten of fewer tokens
 constexpr int kPairMaxStages = 10;
-constexpr size_t kPairSmem = 1024 + kPairRing + (2 * kPairMaxStages + 4) * 8 + 16;
+constexpr size_t kPairSmem = 1024 + kPairRing + (2 * kPairMaxStages + 5) * 8 + 16;
 static_assert(kPairSmem <= kSmemPerSm, "shared memory of one SM");
 
 // What a pair of SMs does at one time: rows [256 RT, ..) for TOKENS tokens from T0 on.
@@ -558,7 +574,8 @@ __global__ void __launch_bounds__(kThreads, 1) int8_pair_kernel(const __grid_con
     uint64_t* empty = full + kPairMaxStages;                                // in both
     uint64_t* acc_full = empty + kPairMaxStages;                            // [2], in both
     uint64_t* acc_empty = acc_full + 2;                                     // [2], in the leader
-    uint32_t* slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
+    uint64_t* last = acc_empty + 2;                                         // in the leader
+    uint32_t* slot = reinterpret_cast<uint32_t*>(last + 1);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = cluster_rank();
@@ -569,8 +586,8 @@ __global__ void __launch_bounds__(kThreads, 1) int8_pair_kernel(const __grid_con
     const int nk = (int)G.kbt;
 
     if (warp == 5) {
-        if (lane < 2 * kPairMaxStages + 4)  // acc_empty: both CTAs' epilogue warps
-            mbar_init(full + lane, lane < 2 * kPairMaxStages + 2 ? 1 : 8);
+        if (lane < 2 * kPairMaxStages + 5)  // acc_empty: both CTAs' epilogue warps
+            mbar_init(full + lane, (lane & ~1) == 2 * kPairMaxStages + 2 ? 8 : 1);
         mbar_init_fence();
     } else if (warp == 4) {
         if (lane < 3) prefetch_map(lane == 0 ? &G.wmap : lane == 1 ? &G.xmap : &G.xmap_part);
@@ -639,11 +656,20 @@ __global__ void __launch_bounds__(kThreads, 1) int8_pair_kernel(const __grid_con
                     }
                     __syncwarp();
                 }
+                if (!ok) break;  // sums that are not whole are not handed on
                 if (elect_one()) mma_commit<2>(accs + 8 * buf);
                 __syncwarp();
             }
             // the MMAs issued last have read their operands before the CTA exits
-            if (nt > 0) mbar_drain(&acc_full[(nt - 1) & 1], (uint32_t)((nt - 1) >> 1) & 1u);
+            if (!ok) {
+                if (elect_one()) mma_commit_here(smem_u32(last));
+                __syncwarp();
+                mbar_drain(last, 0);
+            } else if (nt > 0) {
+                mbar_drain(&acc_full[(nt - 1) & 1], (uint32_t)((nt - 1) >> 1) & 1u);
+            }
+            // where the other CTA may have stopped waiting, the commits' arrivals there get 10 us to land
+            for (int i = 0; i < 10 && *(volatile int*)G.err; i++) __nanosleep(1000);
         }
     } else {
         int64_t nt = 0;

@@ -101,3 +101,32 @@ def test_streamed_rows_stop_where_a_row_does_not_come(cuda, clq, absent, m, k, x
         assert ((total == want[2]) | (total == other)).all()
     assert status(clq) == 0
     assert all(torch.equal(a, b) for a, b in zip(call(), want))
+
+
+@pytest.mark.parametrize("m,n,k", [(24, 4096, 4096), (40, 1024, 16384), (128, 4096, 4096), (64, 512, 40000), (45, 5003, 2051),
+                                   (256, 6144, 4096), (32, 28672, 4096), (512, 4096, 14336), (2048, 4096, 4096),
+                                   (300, 19200, 9000)])
+@pytest.mark.parametrize("onto", [False, True])
+def test_products_write_whole_sums_or_nothing(cuda, clq, absent, m, n, k, onto):
+    """Tiles of one CTA, tiles whose parts of K are a cluster, and SM pairs."""
+    torch = cuda
+    gen = torch.Generator(device="cuda").manual_seed(m)
+
+    def rows(count):
+        c = torch.randint(-128, 128, (count, (k + 15) // 16 * 16), device="cuda", generator=gen, dtype=torch.int16).to(torch.int8)
+        return clq.Int8Rows(c[:, :k], torch.rand(count, device="cuda", generator=gen) + 0.5)
+    x, w, before = rows(m), rows(n), rand(torch, m, n, seed=5)
+
+    def call():
+        out = before.clone()
+        torch.cuda.synchronize()
+        return clq.linear_int8(x, w, out=out, residual=out if onto else None)
+    want = call()
+    assert status(clq) == 0
+    for _ in range(5):
+        absent.expire()
+        got = call()
+        assert clq._lib.STATUS_NAMES[status(clq)] == "CLQ_ERR_TIMEOUT"
+        print(f"{(got == want).double().mean().item():.3f} written")
+        assert ((got == want) | (got == before)).all()
+    assert torch.equal(call(), want)
