@@ -37,7 +37,8 @@ constexpr int kTM = 128;          // weight rows per CTA (the MMA's M)
 constexpr int kKB = 64;           // K elements per stage (one 128-byte swizzle span of fp16)
 constexpr int kStages = 4;
 constexpr int kThreads = 320;     // warps 0-7 dequant/epilogue, 8 copy, 9 MMA
-constexpr uint32_t kWaitLimit = 1u << 26;  // polls before a wait gives up
+constexpr uint32_t kWaitLimit = 1u << 26;       // polls before a wait gives up,
+constexpr uint32_t kWaitNs = 2000u * 1000000u;  // or nanoseconds (a poll may pause for 4 ms)
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {
     return (uint32_t)__cvta_generic_to_shared(p);
@@ -63,9 +64,16 @@ __device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
         : "memory");
     return ok != 0;
 }
+__device__ __forceinline__ uint32_t time_ns() {
+    uint32_t t;
+    asm volatile("mov.u32 %0, %%globaltimer_lo;" : "=r"(t)::"memory");
+    return t;
+}
 // Bounded wait for the phase with PARITY; false (and *err set) when it gives up.
 __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, int* err) {
-    for (uint32_t i = 0; i < kWaitLimit; i++) {
+    if (mbar_test(bar, parity)) return true;
+    const uint32_t start = time_ns();
+    for (uint32_t i = 0; i < kWaitLimit && time_ns() - start < kWaitNs; i++) {
         if (mbar_test(bar, parity)) return true;
         if (*(volatile int*)err) return false;
         if (i > 64) __nanosleep(32);
@@ -76,7 +84,9 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, int* e
 // Bounded wait that ignores the error flag: used before teardown so that copies
 // and MMAs this CTA issued have finished before it exits.
 __device__ __forceinline__ void mbar_drain(uint64_t* bar, uint32_t parity) {
-    for (uint32_t i = 0; i < (1u << 22); i++) {
+    if (mbar_test(bar, parity)) return;
+    const uint32_t start = time_ns();
+    for (uint32_t i = 0; i < (1u << 22) && time_ns() - start < kWaitNs; i++) {
         if (mbar_test(bar, parity)) return;
         if (i > 64) __nanosleep(64);
     }
@@ -824,9 +834,11 @@ __device__ __forceinline__ void tma_box(void* dst, const CUtensorMap* map, int x
 
 // Bounded wait that spins without sleeping (stages are a few hundred cycles).
 __device__ __forceinline__ bool mbar_wait_spin(uint64_t* bar, uint32_t parity, int* err) {
-    for (uint32_t i = 0; i < kWaitLimit; i++) {
+    if (mbar_test(bar, parity)) return true;
+    const uint32_t start = time_ns();
+    for (uint32_t i = 0; i < kWaitLimit && time_ns() - start < kWaitNs; i++) {
         if (mbar_test(bar, parity)) return true;
-        if ((i & 1023) == 1023 && *(volatile int*)err) return false;
+        if (*(volatile int*)err) return false;
     }
     atomicExch(err, CLQ_ERR_TIMEOUT);
     return false;

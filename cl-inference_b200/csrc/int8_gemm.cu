@@ -223,13 +223,12 @@ __device__ __forceinline__ bool elect_one() {
 // barrier, made while other work was under way, found.
 __device__ __forceinline__ bool wait_spin(uint32_t bar, uint32_t parity, int* err, bool ready = false) {
     if (__all_sync(0xffffffffu, ready)) return true;
-    bool ok = false;
-    uint32_t i = 0;
-    for (; i < kWaitLimit; i++) {
-        if ((ok = test(bar, parity))) break;
-        if ((i & 1023) == 1023 && *(volatile int*)err) break;
+    bool ok = test(bar, parity);
+    if (!ok) {  // the pause of a poll has passed
+        const uint32_t start = time_ns();
+        while (!(ok = test(bar, parity)) && !*(volatile int*)err)
+            if (time_ns() - start >= kWaitNs) atomicExch(err, CLQ_ERR_TIMEOUT);
     }
-    if (i == kWaitLimit) atomicExch(err, CLQ_ERR_TIMEOUT);
     return __all_sync(0xffffffffu, ok);
 }
 // A role's place in a ring of n stages: the stage and the parity of its round.

@@ -14,7 +14,9 @@
 namespace clq {
 namespace pipe {
 
-constexpr uint32_t kWaitLimit = 1u << 26;  // polls before a wait gives up (seconds, with the back-off)
+constexpr uint32_t kWaitLimit = 1u << 26;       // polls before a wait gives up,
+constexpr uint32_t kWaitNs = 2000u * 1000000u;  // or nanoseconds, whichever comes first: a poll of a phase
+                                                // that does not come pauses for up to 4 ms
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 
@@ -42,10 +44,17 @@ __device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
         : "memory");
     return ok != 0;
 }
+// The time in nanoseconds, modulo 2^32.
+__device__ __forceinline__ uint32_t time_ns() {
+    uint32_t t;
+    asm volatile("mov.u32 %0, %%globaltimer_lo;" : "=r"(t)::"memory");
+    return t;
+}
 // Bounded wait for the phase with PARITY; false (and *err set) when it gives up.
 __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, int* err) {
     if (mbar_test(bar, parity)) return true;
-    for (uint32_t i = 0; i < kWaitLimit; i++) {
+    const uint32_t start = time_ns();
+    for (uint32_t i = 0; i < kWaitLimit && time_ns() - start < kWaitNs; i++) {
         if (mbar_test(bar, parity)) return true;
         if (*(volatile int*)err) return false;
         if (i > 64) __nanosleep(32);
@@ -56,7 +65,9 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, int* e
 // Bounded wait that ignores the error word: before a CTA exits, so that the
 // copies it issued have landed.
 __device__ __forceinline__ void mbar_drain(uint64_t* bar, uint32_t parity) {
-    for (uint32_t i = 0; i < (1u << 22); i++) {
+    if (mbar_test(bar, parity)) return;
+    const uint32_t start = time_ns();
+    for (uint32_t i = 0; i < (1u << 22) && time_ns() - start < kWaitNs; i++) {
         if (mbar_test(bar, parity)) return;
         if (i > 64) __nanosleep(64);
     }
