@@ -139,7 +139,8 @@ int run_quantize(const QuantRows& q, void* stream) {
 }  // namespace
 
 bool int8_aligned(const Int8Product& p) {
-    return !(((uintptr_t)p.x | (uintptr_t)p.w | (uint64_t)p.ldx | (uint64_t)p.ldw) & 15);
+    const int64_t strides = (p.m > 1 ? p.ldx : 0) | (p.n > 1 ? p.ldw : 0);  // a single row's is never used
+    return !(((uintptr_t)p.x | (uintptr_t)p.w | (uint64_t)strides) & 15);
 }
 
 cudaError_t launch_linear_int8(const Int8Product& p, cudaStream_t s) {

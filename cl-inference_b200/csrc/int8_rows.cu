@@ -849,10 +849,11 @@ cudaError_t launch_loose(const QuantRows& q, cudaStream_t s) {
 // row (the norm 60 us, streamed 70).
 template <typename XT, typename RT, int MODE>
 cudaError_t launch_mode(const QuantRows& q, cudaStream_t s) {
-    const uint64_t bits = (uint64_t)(uintptr_t)q.x | (uint64_t)q.ldx * sizeof(XT) | (uint64_t)(uintptr_t)q.gate |
-                          (uint64_t)q.ldg * sizeof(XT) | (uint64_t)(uintptr_t)q.norm_w | (uint64_t)(uintptr_t)q.res |
-                          (uint64_t)q.ldr * sizeof(RT) | (uint64_t)(uintptr_t)q.res_out | (uint64_t)q.ldro * sizeof(RT) |
-                          (uint64_t)(uintptr_t)q.codes * 2 | (uint64_t)q.ldc * 2 | (uint64_t)q.k * sizeof(XT);
+    const uint64_t strides = (uint64_t)q.ldx * sizeof(XT) | (uint64_t)q.ldg * sizeof(XT) | (uint64_t)q.ldr * sizeof(RT) |
+                             (uint64_t)q.ldro * sizeof(RT) | (uint64_t)q.ldc * 2;
+    const uint64_t bits = (uint64_t)(uintptr_t)q.x | (uint64_t)(uintptr_t)q.gate | (uint64_t)(uintptr_t)q.norm_w |
+                          (uint64_t)(uintptr_t)q.res | (uint64_t)(uintptr_t)q.res_out | (uint64_t)(uintptr_t)q.codes * 2 |
+                          (uint64_t)q.k * sizeof(XT) | (q.m > 1 ? strides : 0);  // a single row's is never used
     if (bits & 15) {
         cudaError_t e = launch_loose<XT, RT, MODE>(q, s);
         if (e == cudaErrorNotSupported) e = try_stream<XT, RT, MODE, true>(q, s);
@@ -890,7 +891,8 @@ template <typename OT>
 cudaError_t launch_dequant(const int8_t* codes, int64_t ldc, const float* scales, int64_t m, int64_t k, void* to,
                            int64_t ldo, cudaStream_t s) {
     OT* out = static_cast<OT*>(to);
-    const uint64_t bits = (uint64_t)(uintptr_t)codes | (uint64_t)ldc | (uint64_t)(uintptr_t)out | (uint64_t)ldo * sizeof(OT);
+    const uint64_t strides = m > 1 ? (uint64_t)ldc | (uint64_t)ldo * sizeof(OT) : 0;  // a single row's is never used
+    const uint64_t bits = (uint64_t)(uintptr_t)codes | (uint64_t)(uintptr_t)out | strides;
     if (bits & 15) {
         const int64_t threads = k * (int64_t)sizeof(OT) / 16 + 1;
         const int T = threads > 128 ? 256 : threads > 32 ? 128 : 32;

@@ -90,11 +90,6 @@ def _here(t, what):
     return device
 
 
-def _ld(t, m, k):
-    """Row stride of an [M, K] matrix; a single row has none to speak of."""
-    return t.stride(0) if m > 1 else (k + 15) // 16 * 16
-
-
 def _on(stream, tensors, call):
     """CALL() with STREAM (a handle) as the current stream, so that what it
     allocates belongs to that stream; TENSORS are kept until STREAM is done."""
@@ -152,12 +147,12 @@ class Int8Rows:
         ldo = k
         if out is not None:
             _writable(out, "out", (m, k), dtype)
-            ldo = _ld(out, m, k)
+            ldo = out.stride(0)
         elif codes.is_contiguous():
             out = torch.empty_like(codes, dtype=dtype)
         else:
             out = codes.new_empty((m, k), dtype=dtype)
-        status = _lib_dequantize(codes.data_ptr(), _ld(codes, m, k), scales.data_ptr(), m, k, out.data_ptr(), code, ldo,
+        status = _lib_dequantize(codes.data_ptr(), codes.stride(0), scales.data_ptr(), m, k, out.data_ptr(), code, ldo,
                                  _stream(device))
         if status:
             _lib.check(status)
@@ -220,12 +215,12 @@ def norm_quantize(x, norm_weight=None, eps=1e-5, residual=None, residual_out=Non
             _writable(residual_out, "residual_out", (m, k), residual.dtype)
             _apart(residual_out, given, "residual_out")
             _apart(residual_out, x, "residual_out")
-        rptr, ldr = residual.data_ptr(), _ld(residual, m, k)
-        optr, ldo = residual_out.data_ptr(), _ld(residual_out, m, k)
+        rptr, ldr = residual.data_ptr(), residual.stride(0)
+        optr, ldo = residual_out.data_ptr(), residual_out.stride(0)
     elif residual_out is not None:
         raise ValueError("residual_out needs a residual")
     q, pitch = _empty_rows(x, m, k)
-    status = _lib_quantize(x.data_ptr(), xtype, m, k, _ld(x, m, k), wptr, eps, rptr, rtype, ldr, optr, ldo, q.codes.data_ptr(),
+    status = _lib_quantize(x.data_ptr(), xtype, m, k, x.stride(0), wptr, eps, rptr, rtype, ldr, optr, ldo, q.codes.data_ptr(),
                            pitch, q.scales.data_ptr(), _stream(_device()))
     if status:
         _lib.check(status)
@@ -246,7 +241,7 @@ def swiglu_quantize(gate, up, stream=None):
     xtype = _type_code(gate.dtype, "gate")
     m, k = gate.shape
     q, pitch = _empty_rows(gate, m, k)
-    status = _lib_swiglu(gate.data_ptr(), _ld(gate, m, k), up.data_ptr(), _ld(up, m, k), xtype, m, k, q.codes.data_ptr(), pitch,
+    status = _lib_swiglu(gate.data_ptr(), gate.stride(0), up.data_ptr(), up.stride(0), xtype, m, k, q.codes.data_ptr(), pitch,
                          q.scales.data_ptr(), _stream(_device()))
     if status:
         _lib.check(status)
@@ -280,7 +275,7 @@ def linear_int8(x, w, out=None, dtype=None, residual=None, stream=None):
     rptr, ldr, ldo = None, 0, n
     if out is not None:
         _writable(out, "out", (m, n), dtype)
-        ldo = _ld(out, m, n)
+        ldo = out.stride(0)
     if residual is not None:
         if out is not None:
             _apart(out, residual, "out")
@@ -288,13 +283,11 @@ def linear_int8(x, w, out=None, dtype=None, residual=None, stream=None):
             residual = _matrix(residual, "residual", (m, n))
             if residual.dtype != torch.float32:
                 raise ValueError(f"residual: float32, not {residual.dtype}")
-        rptr, ldr = residual.data_ptr(), _ld(residual, m, n)
+        rptr, ldr = residual.data_ptr(), residual.stride(0)
     if out is None:
         out = xc.new_empty((m, n), dtype=dtype)
-    single = (k + 15) // 16 * 16  # one row has no stride to speak of
-    status = _lib_linear(xc.data_ptr(), xc.stride(0) if m > 1 else single, x.scales.data_ptr(), m, wc.data_ptr(),
-                         wc.stride(0) if n > 1 else single, w.scales.data_ptr(), n, k, rptr, ldr, out.data_ptr(), code, ldo,
-                         _stream(device))
+    status = _lib_linear(xc.data_ptr(), xc.stride(0), x.scales.data_ptr(), m, wc.data_ptr(), wc.stride(0), w.scales.data_ptr(),
+                         n, k, rptr, ldr, out.data_ptr(), code, ldo, _stream(device))
     if status:
         _lib.check(status)
     return out

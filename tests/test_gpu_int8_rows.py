@@ -136,3 +136,58 @@ def test_norm_of_small_rows_without_epsilon(cuda, clq, k, rtype):
     assert torch.isfinite(fine.scales).all()
     # a weight of zeros leaves nothing to code: an all-zero row
     assert (clq.norm_quantize(h, 0 * g, 0.0).scales == 1).all()
+
+
+def test_the_stride_of_a_single_row_does_not_choose_its_kernel(cuda, clq):
+    """One row, one weight row or both with the base on the 16-byte grid and a stride off it: the same
+    result as with a padded stride, and about its time (the kernels for rows off the grid take twice it)."""
+    torch, lib = cuda, clq._lib.lib
+    k, n = 5123, 4096
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    pitch = (k + 15) // 16 * 16
+    w = torch.randint(-128, 128, (n, pitch), device="cuda", generator=gen, dtype=torch.int16).to(torch.int8)
+    x = torch.randint(-128, 128, (64, pitch), device="cuda", generator=gen, dtype=torch.int16).to(torch.int8)
+    ones = torch.ones(n, device="cuda")
+
+    def product(m, rows, ldx, ldw):
+        out = torch.zeros(m, rows, device="cuda")
+
+        def call():
+            rc = lib.clq_linear_int8_device(x.data_ptr(), ldx, ones.data_ptr(), m, w.data_ptr(), ldw, ones.data_ptr(), rows, k, None,
+                                            0, out.data_ptr(), 0, rows, torch.cuda.current_stream().cuda_stream)
+            assert rc == 0, clq._lib.last_error()
+        return out, call
+
+    values = torch.randn(1, 16384, device="cuda", generator=gen)
+
+    def rows(ldx, ldc):
+        codes, scales = torch.zeros(16384, dtype=torch.int8, device="cuda"), torch.zeros(1, device="cuda")
+
+        def call():
+            assert lib.clq_quantize_rows_device(values.data_ptr(), 0, 1, 16384, ldx, codes.data_ptr(), ldc, scales.data_ptr(),
+                                                torch.cuda.current_stream().cuda_stream) == 0
+        return codes, call
+
+    def micros(call, times=100):
+        call()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            for _ in range(times):
+                call()
+        best = float("inf")
+        for _ in range(5):
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            a.record()
+            graph.replay()
+            b.record()
+            b.synchronize()
+            best = min(best, a.elapsed_time(b) * 1e3 / times)
+        return best
+
+    for padded, tight in ((product(1, n, pitch, pitch), product(1, n, k, pitch)),
+                          (product(64, 1, pitch, pitch), product(64, 1, pitch, k)),
+                          (rows(16384, 16384), rows(16385, 16385))):
+        fast, slow = micros(padded[1]), micros(tight[1])
+        assert torch.equal(padded[0], tight[0]) and padded[0].any()
+        assert slow < 1.4 * fast, (fast, slow)
