@@ -12,7 +12,8 @@ activation, or the output channels of a weight.  The steps of a decoder layer
   y = linear_int8(q, w_down)
 
 Tensors are on the current CUDA device, rows with a unit last stride (others
-are copied) and any row stride.  Work is queued on the current stream, or on
+are copied) and any row stride (of codes and of a product's residual, rows that
+share memory are copied).  Work is queued on the current stream, or on
 STREAM (a cudaStream_t handle): outputs then belong to that stream.
 """
 from . import _lib
@@ -66,6 +67,11 @@ def _matrix(t, what, shape=None):
     return t if t.stride(1) == 1 or t.shape[1] <= 1 else t.contiguous()
 
 
+def _rows_apart(t):
+    """T, or its copy where rows share memory (one row for every token, say)."""
+    return t if t.stride(0) >= t.shape[1] or t.shape[0] <= 1 else t.contiguous()
+
+
 def _vector(t, n, what):
     if not isinstance(t, _t.Tensor) or not t.is_cuda or t.dtype != _t.float32 or t.dim() != 1 or t.shape[0] != n:
         raise ValueError(f"{what}: a CUDA float32 vector of {n}")
@@ -114,7 +120,7 @@ class Int8Rows:
             if codes.dtype != torch.int8:
                 raise ValueError(f"codes: int8, not {codes.dtype}")
             scales = _vector(scales, codes.shape[0], "scales")
-        self.codes, self.scales = codes, scales
+        self.codes, self.scales = _rows_apart(codes), scales
 
     @property
     def shape(self):
@@ -283,6 +289,7 @@ def linear_int8(x, w, out=None, dtype=None, residual=None, stream=None):
             residual = _matrix(residual, "residual", (m, n))
             if residual.dtype != torch.float32:
                 raise ValueError(f"residual: float32, not {residual.dtype}")
+        residual = _rows_apart(residual)
         rptr, ldr = residual.data_ptr(), residual.stride(0)
     if out is None:
         out = xc.new_empty((m, n), dtype=dtype)

@@ -191,3 +191,28 @@ def test_the_stride_of_a_single_row_does_not_choose_its_kernel(cuda, clq):
         fast, slow = micros(padded[1]), micros(tight[1])
         assert torch.equal(padded[0], tight[0]) and padded[0].any()
         assert slow < 1.4 * fast, (fast, slow)
+
+
+def test_rows_that_share_memory_are_read(cuda, clq):
+    """One row for every token, or overlapping windows of a buffer: codes, residuals, values."""
+    torch = cuda
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    row = clq.quantize_rows(torch.randn(1, 160, device="cuda", generator=gen))
+    w = clq.quantize_rows(torch.randn(48, 160, device="cuda", generator=gen))
+    bias = torch.randn(48, device="cuda", generator=gen)
+    for m in (2, 20, 150):
+        x = clq.quantize_rows(torch.randn(m, 160, device="cuda", generator=gen))
+        want = clq.linear_int8(x, w, residual=bias.expand(m, 48).contiguous())
+        assert torch.equal(clq.linear_int8(x, w, residual=bias.expand(m, 48)), want)
+        out = torch.empty(m, 48, device="cuda")
+        assert torch.equal(clq.linear_int8(x, w, out=out, residual=bias.expand(m, 48)), want)
+        same = clq.Int8Rows(row.codes.expand(m, 160), row.scales.expand(m))
+        assert torch.equal(clq.linear_int8(same, w), clq.linear_int8(row, w).expand(m, 48))
+        assert torch.equal(same.dequantize(), row.dequantize().expand(m, 160))
+    line = torch.randn(500, device="cuda", generator=gen)
+    windows = line.unfold(0, 100, 7)
+    assert windows.stride(0) == 7
+    assert torch.equal(clq.quantize_rows(windows).codes, clq.quantize_rows(windows.contiguous()).codes)
+    codes = row.codes[0].unfold(0, 32, 16)
+    wide = clq.Int8Rows(codes, torch.ones(len(codes), device="cuda"))
+    assert torch.equal(clq.linear_int8(wide, wide).double(), codes.double() @ codes.double().t())
