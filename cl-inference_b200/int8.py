@@ -98,10 +98,11 @@ def _here(t, what):
 
 def _on(stream, tensors, call):
     """CALL() with STREAM (a handle) as the current stream, so that what it
-    allocates belongs to that stream; TENSORS are kept until STREAM is done."""
+    allocates belongs to that stream; TENSORS are kept until STREAM is done
+    (CALL refuses what is none, or not on the device)."""
     side = _t.cuda.ExternalStream(stream)
     for t in tensors:
-        if t is not None:
+        if isinstance(t, _t.Tensor) and t.is_cuda:
             t.record_stream(side)
     with _t.cuda.stream(side):
         return call()
@@ -146,7 +147,7 @@ class Int8Rows:
         if codes.get_device() != device:
             _here(codes, "codes")
         if dtype is None:
-            dtype = torch.float32 if out is None else out.dtype
+            dtype = torch.float32 if out is None else getattr(out, "dtype", None)
         code = _types.get(dtype)
         if code is None:
             _type_code(dtype, "dtype")
@@ -274,7 +275,7 @@ def linear_int8(x, w, out=None, dtype=None, residual=None, stream=None):
         _here(xc, "x")
         _here(wc, "w")
     if dtype is None:
-        dtype = torch.float32 if out is None else out.dtype
+        dtype = torch.float32 if out is None else getattr(out, "dtype", None)
     code = _types.get(dtype)
     if code is None:
         _type_code(dtype, "dtype")
@@ -283,12 +284,13 @@ def linear_int8(x, w, out=None, dtype=None, residual=None, stream=None):
         _writable(out, "out", (m, n), dtype)
         ldo = out.stride(0)
     if residual is not None:
-        if out is not None:
-            _apart(out, residual, "out")
+        given = residual
         if not _plain(residual, torch.float32, 2) or residual.shape != (m, n):
             residual = _matrix(residual, "residual", (m, n))
             if residual.dtype != torch.float32:
                 raise ValueError(f"residual: float32, not {residual.dtype}")
+        if out is not None:
+            _apart(out, given, "out")
         residual = _rows_apart(residual)
         rptr, ldr = residual.data_ptr(), residual.stride(0)
     if out is None:

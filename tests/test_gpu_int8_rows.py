@@ -216,3 +216,21 @@ def test_rows_that_share_memory_are_read(cuda, clq):
     codes = row.codes[0].unfold(0, 32, 16)
     wide = clq.Int8Rows(codes, torch.ones(len(codes), device="cuda"))
     assert torch.equal(clq.linear_int8(wide, wide).double(), codes.double() @ codes.double().t())
+
+
+def test_refusals_are_value_errors_whatever_else_is_given(cuda, clq):
+    torch = cuda
+    x = torch.randn(4, 64, device="cuda")
+    q = clq.quantize_rows(x)
+    out, h = torch.empty(4, 4, device="cuda"), torch.cuda.current_stream().cuda_stream
+    for call in (
+        lambda: clq.linear_int8(q, q, out=out, residual="none"), lambda: clq.linear_int8(q, q, out=out, residual=out[0]),
+        lambda: clq.linear_int8(q, q, out=out, residual=torch.zeros(4, 4)),
+        lambda: clq.linear_int8(q, q, out=out, residual=out.t()), lambda: clq.linear_int8(q, q, out="out", stream=h),
+        lambda: clq.linear_int8(q, q, residual=torch.zeros(4, 4), stream=h),
+        lambda: clq.quantize_rows(x.cpu(), stream=h), lambda: clq.quantize_rows([1.0], stream=h),
+        lambda: clq.norm_quantize(x, torch.ones(64), stream=h), lambda: clq.norm_quantize(x, residual=x.cpu(), stream=h),
+        lambda: clq.swiglu_quantize(x, x.cpu(), stream=h), lambda: q.dequantize(out=torch.empty(4, 64), stream=h),
+    ):
+        with pytest.raises(ValueError):
+            call()
