@@ -68,8 +68,10 @@ def _matrix(t, what, shape=None):
 
 
 def _rows_apart(t):
-    """T, or its copy where rows share memory (one row for every token, say)."""
-    return t if t.stride(0) >= t.shape[1] or t.shape[0] <= 1 else t.contiguous()
+    """T and its row stride, or a copy's where rows share memory (one row for every token, say)."""
+    if t.shape[0] > 1 and t.stride(0) < t.shape[1]:
+        t = t.contiguous()
+    return t, t.stride(0)
 
 
 def _vector(t, n, what):
@@ -121,7 +123,7 @@ class Int8Rows:
             if codes.dtype != torch.int8:
                 raise ValueError(f"codes: int8, not {codes.dtype}")
             scales = _vector(scales, codes.shape[0], "scales")
-        self.codes, self.scales = _rows_apart(codes), scales
+        self.codes, self.scales = codes, scales
 
     @property
     def shape(self):
@@ -159,7 +161,10 @@ class Int8Rows:
             out = torch.empty_like(codes, dtype=dtype)
         else:
             out = codes.new_empty((m, k), dtype=dtype)
-        status = _lib_dequantize(codes.data_ptr(), codes.stride(0), scales.data_ptr(), m, k, out.data_ptr(), code, ldo,
+        ldc = codes.stride(0)
+        if ldc < k:
+            codes, ldc = _rows_apart(codes)
+        status = _lib_dequantize(codes.data_ptr(), ldc, scales.data_ptr(), m, k, out.data_ptr(), code, ldo,
                                  _stream(device))
         if status:
             _lib.check(status)
@@ -291,12 +296,19 @@ def linear_int8(x, w, out=None, dtype=None, residual=None, stream=None):
                 raise ValueError(f"residual: float32, not {residual.dtype}")
         if out is not None:
             _apart(out, given, "out")
-        residual = _rows_apart(residual)
-        rptr, ldr = residual.data_ptr(), residual.stride(0)
+        ldr = residual.stride(0)
+        if ldr < n:
+            residual, ldr = _rows_apart(residual)
+        rptr = residual.data_ptr()
     if out is None:
         out = xc.new_empty((m, n), dtype=dtype)
-    status = _lib_linear(xc.data_ptr(), xc.stride(0), x.scales.data_ptr(), m, wc.data_ptr(), wc.stride(0), w.scales.data_ptr(),
-                         n, k, rptr, ldr, out.data_ptr(), code, ldo, _stream(device))
+    ldx, ldw = xc.stride(0), wc.stride(0)
+    if ldx < k:
+        xc, ldx = _rows_apart(xc)
+    if ldw < k:
+        wc, ldw = _rows_apart(wc)
+    status = _lib_linear(xc.data_ptr(), ldx, x.scales.data_ptr(), m, wc.data_ptr(), ldw, w.scales.data_ptr(), n, k, rptr, ldr,
+                         out.data_ptr(), code, ldo, _stream(device))
     if status:
         _lib.check(status)
     return out
