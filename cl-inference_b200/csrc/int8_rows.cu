@@ -820,12 +820,14 @@ cudaError_t launch_rows(const QuantRows& q, cudaStream_t s) {
 }
 
 // Rows off the 16-byte grid, element by element: a warp a row up to 512 elements, then a
-// CTA; few rows over as many threads as help (one of 4097 f32 with norm and residual 2.8
-// us, streamed 4.1).  cudaErrorNotSupported for those that streaming serves better, whose
-// words shared memory puts back together: more than 8192 elements (2048 x 14337
-// SwiGLU bf16 50 us, so 68), and 16-bit rows alone, where an element is a
-// small part of a request (2048 x 7001 bf16 19.9 us, so 23.2; f32 23.0 and 21.9, with
-// norm and residual 65 and 39, SwiGLU 27.7 and 25.7).
+// CTA; few rows (at most one an SM), up to 16384 elements, over as many threads as help (one of
+// 4097 f32 with norm and residual 2.8 us, streamed 4.0).  cudaErrorNotSupported for those
+// that streaming serves better, whose words shared memory puts back together.  Of
+// many rows these are the ones of more than 8192 elements (2048 x 14337 SwiGLU
+// bf16 51 us, so 73); of more than 4096, 16-bit rows alone, where an element is a small
+// part of a request (2048 x 7001 bf16 19.4 us, so 23.6; f32 23.7 and 22.2, with norm
+// and residual 67 and 38); and 16-bit SwiGLU of more than 6144 (7001: 27.7 us, so
+// 29.8; 6143: 24.7 and 22.3).
 template <typename XT, typename RT, int MODE>
 cudaError_t launch_loose(const QuantRows& q, cudaStream_t s) {
     if (q.k <= 512) return launch_held<XT, RT, MODE, true, 32, 16>(q, s);
@@ -838,7 +840,7 @@ cudaError_t launch_loose(const QuantRows& q, cudaStream_t s) {
     }
     if (q.k <= 2048) return launch_held<XT, RT, MODE, true, 128, 16>(q, s);
     if (q.k <= 4096) return launch_held<XT, RT, MODE, true, 256, 16>(q, s);
-    if (q.k > 8192 || (sizeof(XT) == 2 && MODE != kSwiglu && !q.res)) return cudaErrorNotSupported;
+    if (q.k > 8192 || (sizeof(XT) == 2 && (MODE == kSwiglu ? q.k > 6144 : !q.res))) return cudaErrorNotSupported;
     return q.k <= 6144 ? launch_held<XT, RT, MODE, true, 384, 16>(q, s) : launch_held<XT, RT, MODE, true, 512, 16>(q, s);
 }
 
