@@ -784,13 +784,18 @@ int resident_clusters(int splits) {
 // The kernel for a request: the one of least time in microseconds by
 //   max(rounds of resident tiles x columns of K x c, traffic) + rounds x e
 // with c a 128-byte column's time and e a tile's start and end, fitted to every
-// variant at 1024 to 14336 rows and K = 2051 to 14336.  What it decides, at K =
-// 4096 (us; the tile kernel as tokens / parts of K):
-//   24 tokens, 4096 rows    32/4  7.2   32/1  9.1   pair 10.9
-//   128 tokens, 4096 rows   64/2  9.0   64/1  9.5   pair 11.5
-//   256 tokens, 6144 rows   128/1 11.9  pair 13.2   256/2 16.1
-//   256 tokens, 14336 rows  pair 19.6   256/1 21.4  128/1 24.9
-//   512 tokens, 4096 rows, K = 14336:  128/1 29.4  pair 30.4  256/2 31.0
+// variant at 1024 to 14336 rows and K = 2051 to 14336.  For up to 128 tokens c is the
+// issuing loop's: a column of operands in L2 takes 0.18 us for 32 or 64 tokens and 0.19
+// for 128 with four CTAs at work, and 0.18, 0.19 and 0.21 with 144 (the same, so neither
+// a copy's round trip, with seven or more stages in flight, nor L2, which then delivers
+// 16 to 22 TB/s); the MMAs of 128 tokens alone take 0.14.  Those of 256 take 0.27, and
+// their column 0.27 to 0.47 as more SMs work.  What it decides, at K = 4096 (us; the tile
+// kernel as tokens / parts of K):
+//   24 tokens, 4096 rows    32/4  7.5   32/1  8.7   pair 10.7
+//   128 tokens, 4096 rows   64/2  9.0   64/1  9.4   pair 11.3
+//   256 tokens, 6144 rows   128/1 11.8  pair 12.8   256/2 16.3
+//   256 tokens, 14336 rows  pair 19.5   256/1 22.7  128/1 25.3
+//   512 tokens, 4096 rows, K = 14336:  128/1 29.9  pair 30.3  256/2 31.2
 struct Choice {
     int tn, splits, per_sm;  // tn 0: the pair kernel
 };

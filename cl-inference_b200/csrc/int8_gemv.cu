@@ -25,7 +25,7 @@ namespace {
 // 16 bytes of the weight stream, read once: past L1, the whole 256-byte L2
 // line asked for.  Volatile, so that the loads of a batch stay ahead of its
 // MMAs: left to the compiler's order the kernel took 8.3 us for one token at
-// 4096 x 4096, and 4.9 with this one.
+// 4096 x 4096, and 4.9 with this one (4.4 now).
 __device__ __forceinline__ uint4 load_stream(const int8_t* p) {
     uint4 v;
     asm volatile("ld.global.nc.L1::no_allocate.L2::256B.v4.u32 {%0, %1, %2, %3}, [%4];"
@@ -55,8 +55,8 @@ __device__ __forceinline__ uint4 load_tail(const int8_t* row, int64_t k0, int64_
 
 // HI: tokens 8..15 are present.  R: groups of eight weight rows to a CTA.  W:
 // warps.  U: 64-byte columns a warp has in flight.  LOOSE: rows of any address
-// and stride, at twice the loads and their shifts (one token, 4096 x 4096: 9.5 us beside
-// 4.9; 14336 x 4096: 30.3 and 11.9).
+// and stride, at twice the loads and their shifts (one token, 4096 x 4096: 8.9 us beside
+// 4.4; 14336 x 4096: 28.9 and 11.5).
 template <typename OT, int R, bool HI, int W, int U, bool LOOSE>
 __global__ void __launch_bounds__(W * 32, 16 / W) int8_gemv_kernel(const Int8Product P) {
     __shared__ int part[W][R][HI ? 4 : 2][32];
@@ -189,10 +189,10 @@ cudaError_t launch_gv(const Int8Product& p, cudaStream_t s) {
 }
 
 // Few rows: eight to a CTA, K over eight warps, so that every SM has a CTA (1024
-// x 4096 at one token: 2.7 us; 16 rows to a CTA 3.4).  More: 16 to a CTA, which halves
-// what the tokens' rows cost (4096 x 14336: 11.6 us, eight rows 13.6), and from
+// x 4096 at one token: 2.3 us; 16 rows to a CTA 3.2).  More: 16 to a CTA, which halves
+// what the tokens' rows cost (4096 x 14336: 11.1 us, eight rows 16.6), and from
 // four CTAs an SM on four warps, whose longer runs of K keep the loads flowing
-// (14336 x 4096: 11.9 us at one token and 14.2 at sixteen, eight warps 13.2 and 15.5).
+// (14336 x 4096: 11.5 us at one token and 14.2 at sixteen, eight warps 12.9 and 14.5).
 // Off the grid fewer columns are in flight: each takes twice the registers.
 template <typename OT>
 cudaError_t launch_gv_type(const Int8Product& p, cudaStream_t s) {
@@ -208,8 +208,8 @@ cudaError_t launch_gv_type(const Int8Product& p, cudaStream_t s) {
 cudaError_t launch_int8_gemv(const Int8Product& p, cudaStream_t s) {
     if (p.m > 16) return cudaErrorNotSupported;
     // the second half of the tokens' loads costs a fifth of the rate, the tile kernel 2 us more to
-    // start: sixteen tokens at 28672 x 8192 46.6 us here and 40.7 there, at 14336 x 4096 13.8
-    // and 12.9, at 4096 x 4096 5.6 and 7.0
+    // start: sixteen tokens at 28672 x 8192 46.9 us here and 41.5 there, at 14336 x 4096 14.2
+    // and 13.1, at 4096 x 4096 5.5 and 7.2
     if (int8_aligned(p) && p.m > 8 && p.n * p.k > 40 * 1000 * 1000) return cudaErrorNotSupported;
     switch (p.otype) {
     case CLQ_X_F32: return launch_gv_type<float>(p, s);

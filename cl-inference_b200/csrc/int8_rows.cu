@@ -44,7 +44,7 @@ __device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
 // in two parts (t and what its rounding left), so that the relative error stays that of
 // ex2.approx (2^-22); with rcp.approx (2^-23) and four f32 roundings v is within 10
 // roundings of 2^-24.  The library's exponential and an IEEE quotient have 7, and take
-// the kernel, which instructions bound, from 36 us to 58 (2048 rows of 14336 bf16, where
+// the kernel, which instructions bound, from 37 us to 58 (2048 rows of 14336 bf16, where
 // 4 codes of 29 million then differ).  A gate that is NaN or infinite gives NaN or an
 // infinity.
 constexpr float kFarGate = -87.f;
@@ -68,8 +68,8 @@ __device__ __forceinline__ float silu_far(float g, float u) {
     return __fmul_rn(__fmul_rn(__fmul_rn(g, h), u), h);
 }
 // V values of it over the u, the far gates behind one branch: a step seldom holds any
-// (2048 x 14336 bf16 36.4 us; 38.0 with selects in every element, 37.6 with one branch
-// after a thread's whole share).
+// (2048 x 14336 bf16 36.4 us at that step, without far gates 35.8; 38.0 with selects in
+// every element, 37.6 with one branch after a thread's whole share).
 template <int V>
 __device__ __forceinline__ void silu_times(const float (&g)[V], float (&u)[V]) {
     bool far = false;
@@ -342,8 +342,8 @@ constexpr uint32_t kGaveUp = 0xffffffffu;
 constexpr int kStreamStages = 4;
 constexpr int kStreamHeader = 1024;  // barriers and two rows' reductions
 // Threads of a CTA at most: rows off the grid, whose reads are longer, gain by more
-// of them (SwiGLU of 700 x 20001 bf16 26.4 us, with 512 30.4), the others lose (2048 x
-// 14336 37.0, with 1024 39.8).
+// of them (SwiGLU of 700 x 20001 bf16 26.1 us, with 512 31.3), the others lose (2048 x
+// 14336 37.5, with 1024 49).
 constexpr int stream_threads(bool loose) { return loose ? 1024 : 512; }
 constexpr int stream_values(bool loose) { return loose ? 32 : 64; }  // of a thread at most
 
@@ -454,7 +454,7 @@ __device__ __forceinline__ void store_shifted(T* p, int i, int k, const float (&
 // CTA b takes rows b, b + gridDim.x, ..: row r's operands are copied into one of
 // STAGES buffers by the bulk-copy engine while earlier rows are computed, so the
 // memory never waits for the arithmetic (with a CTA per row the two took turns:
-// SwiGLU of 2048 x 14336 bf16 40.6 us, now 35.0, against 22.4 of traffic).  A buffer is
+// SwiGLU of 2048 x 14336 bf16 44 us, so 37.5, against 22.4 of traffic).  A buffer is
 // free once the row's reduction has passed its barrier: every thread then holds
 // its values in registers.  LOOSE: rows of any base, stride and length, put back
 // on the grid from shared memory.  WTS_HELD: the norm weight is kept there too.
@@ -798,7 +798,7 @@ cudaError_t try_stream(const QuantRows& q, cudaStream_t s) {
 
 // One row per CTA (or warp).  Few of them (at most one an SM) wait for one round
 // trip, so they are spread over as many threads as they have chunks, up to 1024; more
-// take 16 values a thread (2048 x 4096 bf16 with an f32 residual: 19.5 us, 32 values 23.7),
+// take 16 values a thread (2048 x 4096 with an f32 residual: f32 19.0 us, 32 values 19.5),
 // short ones a warp, and long ones what fits, 64 values at most.
 template <typename XT, typename RT, int MODE>
 cudaError_t launch_rows(const QuantRows& q, cudaStream_t s) {
@@ -846,9 +846,10 @@ cudaError_t launch_loose(const QuantRows& q, cudaStream_t s) {
 
 // Streams long rows off the 16-byte grid (launch_loose); and, of at least four rows
 // an SM, those whose arithmetic counts beside the traffic: 16-bit rows
-// (2048 x 14336 with an f32 residual and norm 59 us, a CTA per row 77; SwiGLU 35
-// and 41) and SwiGLU of long f32 ones (45 and 49).  f32 rows otherwise keep a CTA per
-// row (the norm 60 us, streamed 70).
+// (2048 x 14336 alone 19 us, a CTA per row 32, with an f32 residual and norm 59.7 and 61.6,
+// SwiGLU 37.5 and 44) and SwiGLU of long f32 ones (2048 x 12288 38.6 us and 41.1, 28672 96 and
+// 107; but 14336, of which an SM holds two rows at a time, 45.5 and 44.6, and 16384 63 and
+// 48).  f32 rows otherwise keep a CTA per row (the norm with its residual 60 us, streamed 78).
 template <typename XT, typename RT, int MODE>
 cudaError_t launch_mode(const QuantRows& q, cudaStream_t s) {
     const uint64_t strides = (uint64_t)q.ldx * sizeof(XT) | (uint64_t)q.ldg * sizeof(XT) | (uint64_t)q.ldr * sizeof(RT) |
